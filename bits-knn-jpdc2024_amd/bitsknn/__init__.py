@@ -37,6 +37,8 @@ EXPORTS = (
     "bitsknn_fused_static_scratch_bytes",
     "bitsknn_fused_l2_topk_f32_static",
     "bitsknn_fused_status",
+    "bitsknn_cross_attention_workspace_bytes",
+    "bitsknn_cross_attention",
 )
 
 
@@ -44,6 +46,19 @@ class FusedTuning(ctypes.Structure):
     """bitsknn_fused_tuning of include/bitsknn.h"""
     _fields_ = [("ranges", ctypes.c_int32), ("first_radius", ctypes.c_int32), ("image", ctypes.c_int32),
                 ("workgroup", ctypes.c_int32), ("reserved", ctypes.c_int32 * 4)]
+
+
+class Rows(ctypes.Structure):
+    """bitsknn_rows of include/bitsknn.h"""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64)]
+
+
+class AttentionShape(ctypes.Structure):
+    """bitsknn_attention_shape of include/bitsknn.h"""
+    _fields_ = [("type", ctypes.c_int32), ("dim", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("query_heads", ctypes.c_int32), ("state_heads", ctypes.c_int32), ("queries", ctypes.c_int32),
+                ("states", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 class BitsKnnError(RuntimeError):
@@ -118,6 +133,11 @@ def lib():
                                                       ctypes.c_int, ctypes.POINTER(FusedTuning), vp, sz, vp]
         L.bitsknn_fused_status.restype = ctypes.c_int
         L.bitsknn_fused_status.argtypes = [vp]
+        rows, shape = ctypes.POINTER(Rows), ctypes.POINTER(AttentionShape)
+        L.bitsknn_cross_attention_workspace_bytes.restype = ctypes.c_size_t
+        L.bitsknn_cross_attention_workspace_bytes.argtypes = [shape]
+        L.bitsknn_cross_attention.restype = ctypes.c_int
+        L.bitsknn_cross_attention.argtypes = [shape, rows, rows, rows, vp, vp, sz, rows, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -339,3 +359,103 @@ def fused_status():
     """Synchronises the current stream and raises BitsKnnError(ERR_INTERNAL) if a fused kernel has
     reported a wait that ran out of polls since the last check."""
     _check(lib().bitsknn_fused_status(_stream()))
+
+
+BF16, FP16 = 0, 1
+
+
+def _attention_type(dtype):
+    import torch
+    assert dtype in (torch.bfloat16, torch.float16), dtype
+    return BF16 if dtype == torch.bfloat16 else FP16
+
+
+def _rows(t):
+    """batch x heads x rows x dim, the last dimension contiguous"""
+    strides = t.stride()
+    assert t.shape[3] <= 1 or strides[3] == 1, "the values of a vector must be contiguous"
+    return Rows(t.data_ptr(), strides[0], strides[1], strides[2])
+
+
+def _attention_shape(queries, state_heads, states, scale):
+    batch, heads, rows, dim = queries.shape
+    return AttentionShape(_attention_type(queries.dtype), dim, batch, heads, state_heads, rows, states,
+                          dim ** -0.5 if scale is None else scale)
+
+
+def _int32(t, shape, device):
+    import torch
+    if t is not None:
+        assert t.dtype == torch.int32 and tuple(t.shape) == shape and t.device == device and t.is_contiguous()
+    return _ptr(t)
+
+
+def _mask_args(mask, batch, states, device):
+    import torch
+    if mask is None:
+        return None, 0
+    assert mask.dtype in (torch.bool, torch.uint8) and tuple(mask.shape) == (batch, states) and mask.device == device
+    assert states <= 1 or mask.stride(1) == 1
+    return _ptr(mask), mask.stride(0) if batch > 1 else 0
+
+
+def _outputs(queries, out, lse):
+    import torch
+    if out is None:
+        out = torch.empty_like(queries)
+    if lse is None:
+        lse = torch.empty(queries.shape[:3], dtype=torch.float32, device=queries.device)
+    assert out.shape == queries.shape and out.dtype == queries.dtype and out.device == queries.device
+    assert lse.shape == queries.shape[:3] and lse.dtype == torch.float32 and lse.is_contiguous()
+    assert lse.device == queries.device
+    return out, lse
+
+
+def _workspace(workspace, need, device):
+    """The caller's bytes, or as many as the call wants."""
+    import torch
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace is None:
+        return None, 0
+    assert workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device
+    return workspace, workspace.numel()
+
+
+def _call(entry, device, *args):
+    """A call of the library on the tensors' own device, on that device's current stream."""
+    import torch
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        _check(entry(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            _check(entry(*args, stream))
+
+
+def cross_attention(queries, keys, values, counts=None, mask=None, scale=None, out=None, lse=None, workspace=None):
+    """Attention of queries (batch x query heads x rows x dim) over keys and values (batch x state heads
+    x states x dim), bfloat16 or float16 device tensors with contiguous vectors (bitsknn_cross_attention).
+    counts: None or batch int32, the states of each sequence; mask: None or batch x states bool / uint8,
+    the states that take part; scale: None -> dim ** -0.5.  workspace: None -> allocated here; or a uint8
+    device tensor (cross_attention_workspace_bytes; a smaller one is used as far as it goes).
+    Returns (out, lse): out like queries, lse batch x query heads x rows float32."""
+    batch, state_heads, states, dim = keys.shape
+    device = queries.device
+    assert queries.is_cuda and keys.device == device and values.device == device
+    assert keys.shape == values.shape and queries.shape[0] == batch and queries.shape[3] == dim
+    assert keys.dtype == queries.dtype and values.dtype == queries.dtype
+    out, lse = _outputs(queries, out, lse)
+    shape = _attention_shape(queries, state_heads, states, scale)
+    need = int(lib().bitsknn_cross_attention_workspace_bytes(shape)) if workspace is None else 0
+    workspace, size = _workspace(workspace, need, device)
+    _call(lib().bitsknn_cross_attention, device, shape, _rows(queries), _rows(keys), _rows(values),
+          _int32(counts, (batch,), device), *_mask_args(mask, batch, states, device), _rows(out), _ptr(lse),
+          _ptr(workspace), size)
+    return out, lse
+
+
+def cross_attention_workspace_bytes(queries, keys):
+    """What cross_attention wants as a workspace for tensors of these shapes."""
+    return int(lib().bitsknn_cross_attention_workspace_bytes(
+        _attention_shape(queries, keys.shape[1], keys.shape[2], 1.0)))

@@ -1,0 +1,164 @@
+// Checks of the attention entry points' arguments: everything is refused before any launch.
+#ifndef BITSKNN_CSRC_ATTENTION_HOST_HPP_
+#define BITSKNN_CSRC_ATTENTION_HOST_HPP_
+
+#include "attention.hpp"
+
+namespace bitsknn
+{
+namespace
+{
+
+// a grid holds fewer than 2^32 threads; 256 threads per workgroup
+constexpr u64 MOST_WORKGROUPS = (1U << 24) - 1;
+
+inline int check_shape(const char* name, const bitsknn_attention_shape& s)
+{
+    if (s.type != BITSKNN_BF16 && s.type != BITSKNN_FP16)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: unknown type %d", name, s.type);
+    }
+    if (s.dim < 1 || s.dim > 256 || s.dim % 8 != 0)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: Unsupported dim: %d (a multiple of 8 up to 256)", name, s.dim);
+    }
+    if (s.batch < 0 || s.queries < 0 || s.states < 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: negative size (batch %d, queries %d, states %d)", name, s.batch,
+                    s.queries, s.states);
+    }
+    if (s.state_heads < 1 || s.query_heads < 1 || s.query_heads % s.state_heads != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: %d query heads do not share %d state heads", name, s.query_heads,
+                    s.state_heads);
+    }
+    if (!(s.scale > 0.0F) || !(s.scale <= 3.402823466e38F))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: scale %g is not positive and finite", name, static_cast<double>(s.scale));
+    }
+    // 32-bit row numbers in the kernels, with room for a tile behind the last row
+    if (static_cast<u64>(s.query_heads / s.state_heads) * static_cast<u64>(s.queries) > 0x7FFF0000ULL ||
+        s.states > 0x7FFF0000 || static_cast<u64>(s.batch) * static_cast<u64>(s.query_heads) > 0x7FFFFFFFULL)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: too many rows", name);
+    }
+    return BITSKNN_OK;
+}
+
+inline int fill_shape(attention_args& a, const bitsknn_attention_shape& s)
+{
+    a.dim = s.dim;
+    a.state_heads = s.state_heads;
+    a.group = s.query_heads / s.state_heads;
+    a.queries_per_head = static_cast<u32>(s.queries);
+    a.rows = static_cast<u32>(a.group) * a.queries_per_head;
+    a.states = static_cast<u32>(s.states);
+    a.scale = s.scale;
+    a.exponent_scale = s.scale * LOG2E;
+    return BITSKNN_OK;
+}
+
+// Whether vectors of `dim` values at these strides (extents above 1 only) never overlap: every stride
+// reaches past all that the smaller ones span.
+inline bool apart(std::int64_t dim, std::int64_t (&stride)[3], const std::int64_t (&extent)[3])
+{
+    std::int64_t s[3];
+    std::int64_t e[3];
+    int n = 0;
+    for (int i = 0; i < 3; ++i)
+    {
+        if (extent[i] > 1)
+        {
+            int at = n++;
+            for (; at > 0 && s[at - 1] > stride[i]; --at)
+            {
+                s[at] = s[at - 1];
+                e[at] = e[at - 1];
+            }
+            s[at] = stride[i];
+            e[at] = extent[i];
+        }
+    }
+    std::int64_t span = dim;
+    for (int i = 0; i < n; ++i)
+    {
+        if (s[i] < span)
+        {
+            return false;
+        }
+        span += s[i] * (e[i] - 1);
+    }
+    return true;
+}
+
+// Strides are looked at where their extent is above 1; the view gets 0 elsewhere.
+inline int check_rows(const char* name, const char* what, const bitsknn_rows& r, const bitsknn_attention_shape& s,
+                      int heads, int rows, bool written, rows_view& view)
+{
+    const std::int64_t extent[3] = {s.batch, heads, rows};
+    std::int64_t stride[3] = {r.batch_stride, r.head_stride, r.row_stride};
+    if (s.batch == 0 || rows == 0)
+    {
+        view = rows_view{nullptr, 0, 0, 0};
+        return BITSKNN_OK;
+    }
+    if (r.data == nullptr)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: %s: null pointer", name, what);
+    }
+    if (reinterpret_cast<std::uintptr_t>(r.data) % 16 != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: %s: vectors must start on 16-byte boundaries", name, what);
+    }
+    for (int i = 0; i < 3; ++i)
+    {
+        stride[i] = extent[i] > 1 ? stride[i] : 0;
+        if (stride[i] < 0 || stride[i] % 8 != 0)
+        {
+            return fail(BITSKNN_ERR_INVALID, "%s: %s: vectors must start on 16-byte boundaries (strides %lld, %lld, %lld)",
+                        name, what, static_cast<long long>(r.batch_stride), static_cast<long long>(r.head_stride),
+                        static_cast<long long>(r.row_stride));
+        }
+        if (stride[i] > (1LL << 44) / extent[i])
+        {
+            return fail(BITSKNN_ERR_INVALID, "%s: %s: stride %lld", name, what, static_cast<long long>(stride[i]));
+        }
+    }
+    if (stride[2] >= 1LL << 24)
+    {
+        // the rows of a tile are addressed in 32 bits
+        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: %s: row stride %lld (below 2^24)", name, what,
+                    static_cast<long long>(stride[2]));
+    }
+    if (written && !apart(s.dim, stride, extent))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: %s: vectors overlap (strides %lld, %lld, %lld)", name, what,
+                    static_cast<long long>(r.batch_stride), static_cast<long long>(r.head_stride),
+                    static_cast<long long>(r.row_stride));
+    }
+    view = rows_view{static_cast<char*>(r.data), stride[0], stride[1], stride[2]};
+    return BITSKNN_OK;
+}
+
+inline int check_mask(const char* name, const bitsknn_attention_shape& s, const void* mask, size_t mask_stride)
+{
+    if (mask != nullptr && s.batch > 1 && mask_stride > (1ULL << 44))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: mask stride %zu", name, mask_stride);
+    }
+    return BITSKNN_OK;
+}
+
+inline int check_workspace(const char* name, const void* workspace)
+{
+    if (reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: the workspace must start on a 16-byte boundary", name);
+    }
+    return BITSKNN_OK;
+}
+
+} // namespace
+} // namespace bitsknn
+
+#endif // BITSKNN_CSRC_ATTENTION_HOST_HPP_

@@ -372,6 +372,64 @@ int bitsknn_fused_l2_topk_f32_static(const float* queries_dim_major, const float
  */
 int bitsknn_fused_status(void* stream);
 
+/*
+ * Attention of query rows over states of another length: what a model does with the states that a
+ * search finds or an encoder leaves behind.  For query row i of head h, with s_j = scale * q_i . k_j
+ * over the states j that take part,
+ *     lse_i = log(sum_j exp(s_j)),   out_i = sum_j exp(s_j - lse_i) v_j
+ * in one pass over the states; no score is written to memory.  A row without any state has out = 0
+ * and lse = -inf.  No counterpart in the reference.
+ *
+ * Vectors are 16-bit floats in batch x heads x rows x dim, every vector contiguous, the other strides
+ * the caller's (bitsknn_rows, in elements; an input's stride may be 0).  query_heads is a multiple of
+ * state_heads: query head h reads state head h / (query_heads / state_heads).
+ *   type           BITSKNN_BF16 or BITSKNN_FP16
+ *   dim            1 <= dim <= 256, a multiple of 8; vectors start on 16-byte boundaries
+ *   queries        rows per query head, may be 0
+ *   states         states per state head, may be 0
+ *   scale          positive and finite
+ *   counts         NULL, or batch int32: sequence b has the states [0, counts[b]) (a count below 0 is
+ *                  0, one above `states` is `states`)
+ *   mask           NULL, or batch rows of `states` bytes, row stride mask_stride: a state whose byte is
+ *                  zero takes no part
+ * Keys and values that take no part are not used, whatever they hold (NaN and infinities too).
+ *   out            as queries, no two vectors overlapping
+ *   lse            NULL, or batch x query_heads x queries floats, contiguous
+ *   workspace      16-byte aligned device memory for partial sums.  Where the rows are too few to fill
+ *                  the GPU the states are cut into ranges that separate workgroups read;
+ *                  bitsknn_cross_attention_workspace_bytes returns what the call wants.  NULL or a
+ *                  smaller workspace is not an error: fewer ranges, down to one.
+ * Products are summed in fp32 and softmax statistics are fp32; the weights exp(s - maximum) are rounded
+ * to the vectors' type for the second product, the result once at the end.
+ * The launch depends on the sizes only, never on counts or mask, so a captured call may be replayed
+ * with other contents.  Calls that overlap in time need workspaces of their own.
+ */
+#define BITSKNN_BF16 0
+#define BITSKNN_FP16 1
+typedef struct bitsknn_rows
+{
+    void* data;
+    int64_t batch_stride;
+    int64_t head_stride;
+    int64_t row_stride;
+} bitsknn_rows;
+typedef struct bitsknn_attention_shape
+{
+    int32_t type;
+    int32_t dim;
+    int32_t batch;
+    int32_t query_heads;
+    int32_t state_heads;
+    int32_t queries;
+    int32_t states;
+    float scale;
+} bitsknn_attention_shape;
+size_t bitsknn_cross_attention_workspace_bytes(const bitsknn_attention_shape* shape);
+int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_rows* queries,
+                            const bitsknn_rows* keys, const bitsknn_rows* values, const int32_t* counts,
+                            const uint8_t* mask, size_t mask_stride, const bitsknn_rows* out, float* lse,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

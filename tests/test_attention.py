@@ -1,0 +1,100 @@
+"""What the attention entry points refuse, and with which message: checked before any pointer is read
+and before any HIP call, so it runs without a GPU."""
+import ctypes
+
+import pytest
+
+
+def _rows(bk, batch_stride=1 << 20, head_stride=1 << 10, row_stride=64, data=1 << 20):
+    return bk.Rows(data, batch_stride, head_stride, row_stride)
+
+
+def _shape(bk, **kw):
+    values = dict(type=bk.BF16, dim=64, batch=2, query_heads=4, state_heads=2, queries=3, states=16, scale=0.125)
+    values.update(kw)
+    return bk.AttentionShape(*values.values())
+
+
+def _attend(bk, shape=None, queries=None, keys=None, values=None, out=None, mask=None, mask_stride=0, workspace=None):
+    L = bk.lib()
+    one = _rows(bk)
+    status = L.bitsknn_cross_attention(shape or _shape(bk), queries or one, keys or one, values or one, None, mask,
+                                       mask_stride, out or one, None, workspace, 0, None)
+    return status, L.bitsknn_last_error().decode()
+
+
+SHAPES = [
+    (dict(type=2), "UNSUPPORTED", "unknown type 2"),
+    (dict(dim=0), "UNSUPPORTED", "Unsupported dim: 0"),
+    (dict(dim=60), "UNSUPPORTED", "Unsupported dim: 60"),
+    (dict(dim=264), "UNSUPPORTED", "Unsupported dim: 264"),
+    (dict(batch=-1), "INVALID", "negative size"),
+    (dict(queries=-1), "INVALID", "negative size"),
+    (dict(states=-7), "INVALID", "negative size"),
+    (dict(state_heads=0), "INVALID", "do not share"),
+    (dict(query_heads=3), "INVALID", "3 query heads do not share 2 state heads"),
+    (dict(query_heads=0), "INVALID", "do not share"),
+    (dict(scale=0.0), "INVALID", "not positive and finite"),
+    (dict(scale=-1.0), "INVALID", "not positive and finite"),
+    (dict(scale=float("inf")), "INVALID", "not positive and finite"),
+    (dict(scale=float("nan")), "INVALID", "not positive and finite"),
+    (dict(queries=1 << 30, query_heads=8), "UNSUPPORTED", "too many rows"),
+    (dict(states=0x7FFFFFFF), "UNSUPPORTED", "too many rows"),
+]
+
+
+@pytest.mark.parametrize("change,code,message", SHAPES)
+def test_shapes_that_are_refused(bk, change, code, message):
+    status, text = _attend(bk, _shape(bk, **change))
+    assert status == getattr(bk, "ERR_" + code) and message in text, text
+    assert bk.lib().bitsknn_cross_attention_workspace_bytes(_shape(bk, **change)) == 0
+
+
+ROWS = [
+    (dict(data=0), "null pointer"),
+    (dict(data=(1 << 20) + 8), "16-byte boundaries"),
+    (dict(row_stride=68), "16-byte boundaries"),
+    (dict(head_stride=-64), "16-byte boundaries"),
+    (dict(batch_stride=4), "16-byte boundaries"),
+    (dict(batch_stride=1 << 44), "stride"),
+    (dict(row_stride=1 << 24), "row stride"),
+]
+
+
+@pytest.mark.parametrize("which", ["queries", "keys", "values", "out"])
+@pytest.mark.parametrize("change,message", ROWS)
+def test_vectors_that_are_refused(bk, which, change, message):
+    status, text = _attend(bk, **{which: _rows(bk, **change)})
+    assert status in (bk.ERR_INVALID, bk.ERR_UNSUPPORTED) and message in text and which in text, text
+
+
+@pytest.mark.parametrize("change", [dict(row_stride=0), dict(head_stride=0), dict(batch_stride=0), dict(row_stride=56),
+                                    dict(head_stride=128), dict(row_stride=1 << 10), dict(batch_stride=1 << 10)])
+def test_outputs_that_overlap_are_refused(bk, change):
+    status, text = _attend(bk, out=_rows(bk, **change))
+    assert status == bk.ERR_INVALID and "out: vectors overlap" in text, text
+
+
+def test_other_refusals(bk):
+    L = bk.lib()
+    one = _rows(bk)
+    assert L.bitsknn_cross_attention(None, one, one, one, None, None, 0, one, None, None, 0, None) == bk.ERR_INVALID
+    assert L.bitsknn_cross_attention(_shape(bk), one, None, one, None, None, 0, one, None, None, 0, None) == bk.ERR_INVALID
+    status, text = _attend(bk, workspace=ctypes.c_void_p(8))
+    assert status == bk.ERR_INVALID and "workspace" in text
+    status, text = _attend(bk, mask=ctypes.c_void_p(64), mask_stride=1 << 60)
+    assert status == bk.ERR_INVALID and "mask stride" in text
+    # nothing to do: no launch, whatever the pointers
+    empty = bk.Rows(None, 0, 0, 0)
+    assert _attend(bk, _shape(bk, batch=0), empty, empty, empty, empty)[0] == bk.OK
+    assert _attend(bk, _shape(bk, queries=0), empty, one, one, empty)[0] == bk.OK
+
+
+def test_workspace_sizes(bk):
+    """Ranges only where the rows leave most of the GPU idle, each at least four tiles of 64 states."""
+    size = bk.lib().bitsknn_cross_attention_workspace_bytes
+    assert size(_shape(bk, states=255)) == 0
+    assert size(_shape(bk, batch=64, query_heads=64, state_heads=64, states=1 << 20)) == 0
+    few = size(_shape(bk, states=4096))
+    assert 0 < few <= 64 * 2 * 4 * 3 * (64 * 4 + 8)
+    assert size(_shape(bk, states=1 << 20)) >= few
