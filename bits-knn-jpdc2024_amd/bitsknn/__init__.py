@@ -8,6 +8,7 @@ message.
 """
 import ctypes
 import os
+from typing import NamedTuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libbitsknn.so")
@@ -39,6 +40,9 @@ EXPORTS = (
     "bitsknn_fused_status",
     "bitsknn_cross_attention_workspace_bytes",
     "bitsknn_cross_attention",
+    "bitsknn_cache_store",
+    "bitsknn_cached_attention_workspace_bytes",
+    "bitsknn_cached_attention",
 )
 
 
@@ -59,6 +63,13 @@ class AttentionShape(ctypes.Structure):
     _fields_ = [("type", ctypes.c_int32), ("dim", ctypes.c_int32), ("batch", ctypes.c_int32),
                 ("query_heads", ctypes.c_int32), ("state_heads", ctypes.c_int32), ("queries", ctypes.c_int32),
                 ("states", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class Cache(ctypes.Structure):
+    """bitsknn_state_cache of include/bitsknn.h"""
+    _fields_ = [("key_codes", ctypes.c_void_p), ("value_codes", ctypes.c_void_p), ("key_scales", ctypes.c_void_p),
+                ("value_scales", ctypes.c_void_p), ("block_counts", ctypes.c_void_p), ("blocks", ctypes.c_int32),
+                ("state_heads", ctypes.c_int32), ("block", ctypes.c_int32), ("dim", ctypes.c_int32)]
 
 
 class BitsKnnError(RuntimeError):
@@ -138,6 +149,13 @@ def lib():
         L.bitsknn_cross_attention_workspace_bytes.argtypes = [shape]
         L.bitsknn_cross_attention.restype = ctypes.c_int
         L.bitsknn_cross_attention.argtypes = [shape, rows, rows, rows, vp, vp, sz, rows, vp, vp, sz, vp]
+        cache = ctypes.POINTER(Cache)
+        L.bitsknn_cache_store.restype = ctypes.c_int
+        L.bitsknn_cache_store.argtypes = [cache, i32, i32, i32, rows, rows, vp, vp, sz, vp]
+        L.bitsknn_cached_attention_workspace_bytes.restype = ctypes.c_size_t
+        L.bitsknn_cached_attention_workspace_bytes.argtypes = [shape]
+        L.bitsknn_cached_attention.restype = ctypes.c_int
+        L.bitsknn_cached_attention.argtypes = [shape, rows, cache, vp, sz, vp, rows, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -361,7 +379,7 @@ def fused_status():
     _check(lib().bitsknn_fused_status(_stream()))
 
 
-BF16, FP16 = 0, 1
+BF16, FP16, F32 = 0, 1, 2
 
 
 def _attention_type(dtype):
@@ -459,3 +477,84 @@ def cross_attention_workspace_bytes(queries, keys):
     """What cross_attention wants as a workspace for tensors of these shapes."""
     return int(lib().bitsknn_cross_attention_workspace_bytes(
         _attention_shape(queries, keys.shape[1], keys.shape[2], 1.0)))
+
+
+class StateCache(NamedTuple):
+    """States in 8 bits, in blocks (bitsknn_state_cache): e4m3 codes (uint8 or float8_e4m3fn, blocks x
+    state heads x block x dim), float32 scales (blocks x state heads), int32 states per block."""
+    key_codes: object
+    value_codes: object
+    key_scales: object
+    value_scales: object
+    block_counts: object
+
+
+def state_cache(blocks, state_heads, block, dim, device="cuda"):
+    """An empty cache."""
+    import torch
+    codes = [torch.zeros((blocks, state_heads, block, dim), dtype=torch.uint8, device=device) for _ in range(2)]
+    scales = [torch.ones((blocks, state_heads), dtype=torch.float32, device=device) for _ in range(2)]
+    return StateCache(*codes, *scales, torch.zeros(blocks, dtype=torch.int32, device=device))
+
+
+def _cache_args(cache, device):
+    import torch
+    blocks, state_heads, block, dim = cache.key_codes.shape
+    for codes in (cache.key_codes, cache.value_codes):
+        assert codes.dtype in (torch.uint8, torch.float8_e4m3fn) and codes.is_contiguous()
+        assert codes.shape == cache.key_codes.shape and codes.device == device
+    for scales in (cache.key_scales, cache.value_scales):
+        assert scales.dtype == torch.float32 and scales.is_contiguous() and scales.device == device
+        assert tuple(scales.shape) == (blocks, state_heads)
+    return Cache(cache.key_codes.data_ptr(), cache.value_codes.data_ptr(), cache.key_scales.data_ptr(),
+                 cache.value_scales.data_ptr(), _int32(cache.block_counts, (blocks,), device), blocks, state_heads,
+                 block, dim)
+
+
+def _table_args(table, batch, device):
+    import torch
+    assert table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == batch and table.device == device
+    assert table.shape[1] <= 1 or table.stride(1) == 1
+    return _ptr(table), table.stride(0) if batch > 1 else 0
+
+
+def cache_store(cache, keys, values, table, counts=None):
+    """Writes keys and values (batch x state heads x states x dim; bfloat16, float16 or float32) into the
+    blocks of the cache that table (batch x at least ceil(states / block) int32) names
+    (bitsknn_cache_store).  counts: None or batch int32.  Returns the cache."""
+    import torch
+    batch, state_heads, states, dim = keys.shape
+    device = keys.device
+    block = cache.key_codes.shape[2]
+    assert keys.is_cuda and values.shape == keys.shape and values.device == device and values.dtype == keys.dtype
+    assert (state_heads, dim) == (cache.key_codes.shape[1], cache.key_codes.shape[3])
+    assert table.shape[1] * block >= states, "the table has too few entries for the states"
+    kind = F32 if keys.dtype == torch.float32 else _attention_type(keys.dtype)
+    _call(lib().bitsknn_cache_store, device, _cache_args(cache, device), kind, batch, states, _rows(keys),
+          _rows(values), _int32(counts, (batch,), device), *_table_args(table, batch, device))
+    return cache
+
+
+def cached_attention(queries, cache, table, counts=None, scale=None, out=None, lse=None, workspace=None):
+    """cross_attention over the states of a cache (bitsknn_cached_attention): table (batch x entries int32)
+    names each sequence's blocks, an entry outside the cache's blocks none; counts: None, or batch int32,
+    the places of each sequence that take part.  Returns (out, lse)."""
+    batch, _, _, dim = queries.shape
+    device = queries.device
+    _, state_heads, block, cache_dim = cache.key_codes.shape
+    assert queries.is_cuda and cache_dim == dim
+    out, lse = _outputs(queries, out, lse)
+    shape = _attention_shape(queries, state_heads, table.shape[1] * block, scale)
+    need = int(lib().bitsknn_cached_attention_workspace_bytes(shape)) if workspace is None else 0
+    workspace, size = _workspace(workspace, need, device)
+    _call(lib().bitsknn_cached_attention, device, shape, _rows(queries), _cache_args(cache, device),
+          *_table_args(table, batch, device), _int32(counts, (batch,), device), _rows(out), _ptr(lse), _ptr(workspace),
+          size)
+    return out, lse
+
+
+def cached_attention_workspace_bytes(queries, cache, entries):
+    """What cached_attention wants as a workspace for tables of this many entries per sequence."""
+    _, state_heads, block, _ = cache.key_codes.shape
+    return int(lib().bitsknn_cached_attention_workspace_bytes(
+        _attention_shape(queries, state_heads, entries * block, 1.0)))

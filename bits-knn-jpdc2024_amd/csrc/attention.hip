@@ -532,3 +532,43 @@ extern "C" int bitsknn_cross_attention(const bitsknn_attention_shape* shape, con
     a.lse = lse;
     return run<false>(a, s, workspace, workspace_bytes, stream);
 }
+
+extern "C" size_t bitsknn_cached_attention_workspace_bytes(const bitsknn_attention_shape* shape)
+{
+    return bitsknn_cross_attention_workspace_bytes(shape);
+}
+
+extern "C" int bitsknn_cached_attention(const bitsknn_attention_shape* shape, const bitsknn_rows* queries,
+                                        const bitsknn_state_cache* cache, const int32_t* table, size_t table_stride,
+                                        const int32_t* counts, const bitsknn_rows* out, float* lse, void* workspace,
+                                        size_t workspace_bytes, void* stream)
+{
+    using namespace bitsknn;
+    clear_error();
+    const char* name = "bitsknn_cached_attention";
+    if (shape == nullptr || queries == nullptr || cache == nullptr || out == nullptr)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: null pointer", name);
+    }
+    const bitsknn_attention_shape& s = *shape;
+    attention_args a = {};
+    int status = check_shape(name, s);
+    status = status != BITSKNN_OK ? status : fill_shape(a, s);
+    status = status != BITSKNN_OK ? status : check_rows(name, "queries", *queries, s, s.query_heads, s.queries, false, a.queries);
+    status = status != BITSKNN_OK ? status : check_rows(name, "out", *out, s, s.query_heads, s.queries, true, a.out);
+    status = status != BITSKNN_OK ? status : check_cache(name, cache, a.cache);
+    status = status != BITSKNN_OK ? status : check_table(name, table, table_stride, s.batch, s.states, a.cache);
+    status = status != BITSKNN_OK ? status : check_workspace(name, workspace);
+    if (status == BITSKNN_OK && (cache->dim != s.dim || cache->state_heads != s.state_heads))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: a cache of %d heads x %d, queries for %d x %d", name, cache->state_heads,
+                    cache->dim, s.state_heads, s.dim);
+    }
+    if (status != BITSKNN_OK || s.batch == 0 || s.queries == 0)
+    {
+        return status;
+    }
+    a.counts = counts;
+    a.lse = lse;
+    return run<true>(a, s, workspace, workspace_bytes, stream);
+}

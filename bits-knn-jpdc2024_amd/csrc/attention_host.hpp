@@ -149,6 +149,63 @@ inline int check_mask(const char* name, const bitsknn_attention_shape& s, const 
     return BITSKNN_OK;
 }
 
+inline int check_cache(const char* name, const bitsknn_state_cache* c, cache_view& view)
+{
+    if (c == nullptr)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: null pointer", name);
+    }
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128 && c->block != 256)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "Unsupported block: %d (16, 32, 64, 128 or 256 states)", c->block);
+    }
+    if (c->dim < 1 || c->dim > 256 || c->dim % 8 != 0)
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: Unsupported dim: %d (a multiple of 8 up to 256)", name, c->dim);
+    }
+    if (c->blocks < 0 || c->state_heads < 1)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: a cache of %d blocks, %d heads", name, c->blocks, c->state_heads);
+    }
+    if (c->blocks > 0 && (c->key_codes == nullptr || c->value_codes == nullptr || c->key_scales == nullptr ||
+                          c->value_scales == nullptr || c->block_counts == nullptr))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: cache: null pointer", name);
+    }
+    if (reinterpret_cast<std::uintptr_t>(c->key_codes) % 16 != 0 || reinterpret_cast<std::uintptr_t>(c->value_codes) % 16 != 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: cache: codes must start on 16-byte boundaries", name);
+    }
+    view.key_codes = c->key_codes;
+    view.value_codes = c->value_codes;
+    view.key_scales = c->key_scales;
+    view.value_scales = c->value_scales;
+    view.block_counts = c->block_counts;
+    view.blocks = static_cast<u32>(c->blocks);
+    view.block_shift = 4;
+    while ((1 << view.block_shift) < c->block)
+    {
+        ++view.block_shift;
+    }
+    return BITSKNN_OK;
+}
+
+inline int check_table(const char* name, const std::int32_t* table, size_t table_stride, std::int32_t batch,
+                       std::int32_t states, cache_view& view)
+{
+    if (table == nullptr && batch > 0 && states > 0)
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: table: null pointer", name);
+    }
+    if (batch > 1 && table_stride > (1ULL << 32))
+    {
+        return fail(BITSKNN_ERR_INVALID, "%s: table stride %zu", name, table_stride);
+    }
+    view.table = table;
+    view.table_stride = batch > 1 ? static_cast<std::int64_t>(table_stride) : 0;
+    return BITSKNN_OK;
+}
+
 inline int check_workspace(const char* name, const void* workspace)
 {
     if (reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0)

@@ -430,6 +430,66 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
                             const uint8_t* mask, size_t mask_stride, const bitsknn_rows* out, float* lse,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * A cache of states in 8 bits: keys and values as e4m3 codes (OCP: sign, 4 exponent bits, 3 mantissa
+ * bits, largest 448) in blocks of `block` states, with one scale for each block and state head; a code
+ * stands for its value times the scale.  The caller owns the arrays:
+ *   key_codes, value_codes    blocks x state_heads x block x dim bytes, 16-byte aligned
+ *   key_scales, value_scales  blocks x state_heads floats
+ *   block_counts              blocks int32: how many states a block holds (its first ones)
+ * block is 16, 32, 64, 128 or 256; dim as for bitsknn_cross_attention.  No counterpart in the reference.
+ *
+ * A block table names blocks: batch rows of int32, row stride table_stride, entry t of a row is the
+ * block of the row's states [t * block, (t + 1) * block).  An entry outside [0, blocks) names none: it
+ * is passed over when storing and holds no state when reading.  So the labels of a top-k (INT32_MAX
+ * behind the last candidate) are a table as they stand: a search for the nearest blocks hands its
+ * labels to the attention.
+ */
+typedef struct bitsknn_state_cache
+{
+    uint8_t* key_codes;
+    uint8_t* value_codes;
+    float* key_scales;
+    float* value_scales;
+    int32_t* block_counts;
+    int32_t blocks;
+    int32_t state_heads;
+    int32_t block;
+    int32_t dim;
+} bitsknn_state_cache;
+
+/*
+ * Writes states into the blocks that the table names: for each block and head the scale is the smallest
+ * power of two that is at least (largest finite magnitude / 448), and at least 2^-126, so that dividing
+ * by it is exact and each value is rounded once, to the nearest e4m3 number (ties to even).  A NaN or an
+ * infinity becomes the NaN code.  block_counts of the written blocks is set.
+ *   type           BITSKNN_BF16, BITSKNN_FP16 or BITSKNN_F32: what keys and values hold
+ *   keys, values   batch x cache->state_heads x states x cache->dim
+ *   counts         NULL, or batch int32 as for bitsknn_cross_attention
+ *   table          batch rows of at least ceil(states / block) entries
+ * Blocks behind a sequence's count, and the places of a block behind its last state, are left as they
+ * were.  A table must not name a block twice (which of the writers a block then holds the states of,
+ * is not defined).
+ */
+#define BITSKNN_F32 2
+int bitsknn_cache_store(const bitsknn_state_cache* cache, int32_t type, int32_t batch, int32_t states,
+                        const bitsknn_rows* keys, const bitsknn_rows* values, const int32_t* counts,
+                        const int32_t* table, size_t table_stride, void* stream);
+
+/*
+ * bitsknn_cross_attention over the states of a cache: shape->states places per sequence, in the blocks
+ * that ceil(states / block) entries of the table name; place j takes part if j < counts[b] (where counts
+ * is given), its block is named, and its place in the block is below the block's block_counts.  A block
+ * named twice counts twice.  shape->state_heads and shape->dim are the cache's; scales as stored or any
+ * others.  The codes are multiplied as they stand and the scales are applied in fp32.  Arguments else,
+ * workspace, results and errors as for bitsknn_cross_attention.
+ */
+size_t bitsknn_cached_attention_workspace_bytes(const bitsknn_attention_shape* shape);
+int bitsknn_cached_attention(const bitsknn_attention_shape* shape, const bitsknn_rows* queries,
+                             const bitsknn_state_cache* cache, const int32_t* table, size_t table_stride,
+                             const int32_t* counts, const bitsknn_rows* out, float* lse, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

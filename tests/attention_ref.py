@@ -71,6 +71,14 @@ def attention(queries, keys, values, scale, keep, value_step=None):
 
 
 def check(got, want, bound, what):
+    """got is within bound of want.  Where the type of got ends, rounding to nearest gives infinity: fp16's
+    largest is 65504 and its next step would end at 65536, so a value of 65520 and more is infinite."""
+    if got.dtype == torch.float16:
+        bound = bound.expand_as(want)
+        over = want.abs() >= 65520
+        either = ((want.abs() - 65520).abs() <= bound) & want.isfinite()
+        side = torch.where(either, got.detach().cpu().isinf(), over)
+        want = torch.where(side, want.sign() * math.inf, want)
     got = got.detach().cpu().double()
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert torch.equal(got.isinf(), want.isinf()), what

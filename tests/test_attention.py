@@ -98,3 +98,85 @@ def test_workspace_sizes(bk):
     few = size(_shape(bk, states=4096))
     assert 0 < few <= 64 * 2 * 4 * 3 * (64 * 4 + 8)
     assert size(_shape(bk, states=1 << 20)) >= few
+
+
+# ---- the cache ------------------------------------------------------------------------------------
+
+
+def _cache(bk, **kw):
+    values = dict(key_codes=1 << 20, value_codes=1 << 21, key_scales=1 << 22, value_scales=1 << 23,
+                  block_counts=1 << 24, blocks=8, state_heads=2, block=16, dim=64)
+    values.update(kw)
+    return bk.Cache(*values.values())
+
+
+def _store(bk, cache=None, type=0, batch=2, states=20, keys=None, values=None, table=64, table_stride=2):
+    L = bk.lib()
+    one = _rows(bk)
+    status = L.bitsknn_cache_store(cache or _cache(bk), type, batch, states, keys or one, values or one, None,
+                                   ctypes.c_void_p(table), table_stride, None)
+    return status, L.bitsknn_last_error().decode()
+
+
+def _read(bk, cache=None, shape=None, queries=None, out=None, table=64, table_stride=2, workspace=None):
+    L = bk.lib()
+    one = _rows(bk)
+    status = L.bitsknn_cached_attention(shape or _shape(bk), queries or one, cache or _cache(bk), ctypes.c_void_p(table),
+                                        table_stride, None, out or one, None, workspace, 0, None)
+    return status, L.bitsknn_last_error().decode()
+
+
+CACHES = [
+    (dict(block=0), "UNSUPPORTED", "Unsupported block: 0"),
+    (dict(block=24), "UNSUPPORTED", "Unsupported block: 24"),
+    (dict(block=512), "UNSUPPORTED", "Unsupported block: 512"),
+    (dict(dim=0), "UNSUPPORTED", "Unsupported dim: 0"),
+    (dict(dim=65), "UNSUPPORTED", "Unsupported dim: 65"),
+    (dict(dim=264), "UNSUPPORTED", "Unsupported dim: 264"),
+    (dict(blocks=-1), "INVALID", "a cache of -1 blocks"),
+    (dict(state_heads=0), "INVALID", "0 heads"),
+    (dict(key_codes=0), "INVALID", "cache: null pointer"),
+    (dict(value_scales=0), "INVALID", "cache: null pointer"),
+    (dict(block_counts=0), "INVALID", "cache: null pointer"),
+    (dict(key_codes=(1 << 20) + 8), "INVALID", "16-byte boundaries"),
+    (dict(value_codes=(1 << 20) + 4), "INVALID", "16-byte boundaries"),
+]
+
+
+@pytest.mark.parametrize("change,code,message", CACHES)
+@pytest.mark.parametrize("entry", [_store, _read])
+def test_caches_that_are_refused(bk, entry, change, code, message):
+    status, text = entry(bk, _cache(bk, **change))
+    assert status == getattr(bk, "ERR_" + code) and message in text, text
+
+
+def test_store_refusals(bk):
+    assert _store(bk, type=3) == (bk.ERR_UNSUPPORTED, "bitsknn_cache_store: unknown type 3")
+    assert _store(bk, batch=-1)[0] == bk.ERR_INVALID
+    assert _store(bk, states=-1)[0] == bk.ERR_INVALID
+    status, text = _store(bk, table=None)
+    assert status == bk.ERR_INVALID and "table: null pointer" in text
+    status, text = _store(bk, table_stride=1 << 40)
+    assert status == bk.ERR_INVALID and "table stride" in text
+    for change, message in ROWS:
+        for which in ("keys", "values"):
+            status, text = _store(bk, **{which: _rows(bk, **change)})
+            assert status != bk.OK and message in text and which in text
+    # nothing to do
+    assert _store(bk, batch=0)[0] == bk.OK and _store(bk, states=0)[0] == bk.OK
+    assert _store(bk, _cache(bk, blocks=0))[0] == bk.OK
+
+
+def test_cached_attention_refusals(bk):
+    for change, code, message in SHAPES:
+        status, text = _read(bk, shape=_shape(bk, **change))
+        assert status == getattr(bk, "ERR_" + code) and message in text, text
+    assert _read(bk, shape=_shape(bk, dim=128))[0] == bk.ERR_INVALID
+    assert _read(bk, shape=_shape(bk, query_heads=3, state_heads=1))[0] == bk.ERR_INVALID
+    status, text = _read(bk, table=None)
+    assert status == bk.ERR_INVALID and "table: null pointer" in text
+    assert _read(bk, table_stride=1 << 40)[0] == bk.ERR_INVALID
+    assert _read(bk, workspace=ctypes.c_void_p(4))[0] == bk.ERR_INVALID
+    status, text = _read(bk, out=_rows(bk, row_stride=0))
+    assert status == bk.ERR_INVALID and "out: vectors overlap" in text
+    assert _read(bk, shape=_shape(bk, queries=0), queries=bk.Rows(), out=bk.Rows())[0] == bk.OK
