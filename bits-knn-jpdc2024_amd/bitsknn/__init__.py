@@ -40,6 +40,8 @@ EXPORTS = (
     "bitsknn_fused_status",
     "bitsknn_cross_attention_workspace_bytes",
     "bitsknn_cross_attention",
+    "bitsknn_cross_attention_backward_workspace_bytes",
+    "bitsknn_cross_attention_backward",
     "bitsknn_cache_store",
     "bitsknn_cached_attention_workspace_bytes",
     "bitsknn_cached_attention",
@@ -149,6 +151,10 @@ def lib():
         L.bitsknn_cross_attention_workspace_bytes.argtypes = [shape]
         L.bitsknn_cross_attention.restype = ctypes.c_int
         L.bitsknn_cross_attention.argtypes = [shape, rows, rows, rows, vp, vp, sz, rows, vp, vp, sz, vp]
+        L.bitsknn_cross_attention_backward_workspace_bytes.restype = ctypes.c_size_t
+        L.bitsknn_cross_attention_backward_workspace_bytes.argtypes = [shape]
+        L.bitsknn_cross_attention_backward.restype = ctypes.c_int
+        L.bitsknn_cross_attention_backward.argtypes = [shape] + [rows] * 5 + [vp, vp, vp, sz] + [rows] * 3 + [vp, sz, vp]
         cache = ctypes.POINTER(Cache)
         L.bitsknn_cache_store.restype = ctypes.c_int
         L.bitsknn_cache_store.argtypes = [cache, i32, i32, i32, rows, rows, vp, vp, sz, vp]
@@ -476,6 +482,42 @@ def cross_attention(queries, keys, values, counts=None, mask=None, scale=None, o
 def cross_attention_workspace_bytes(queries, keys):
     """What cross_attention wants as a workspace for tensors of these shapes."""
     return int(lib().bitsknn_cross_attention_workspace_bytes(
+        _attention_shape(queries, keys.shape[1], keys.shape[2], 1.0)))
+
+
+def cross_attention_backward(grad_out, queries, keys, values, out, lse, counts=None, mask=None, scale=None,
+                             grad_queries=None, grad_keys=None, grad_values=None, workspace=None):
+    """Gradients of cross_attention's out with respect to queries, keys and values, given the gradient of
+    out and what the forward call read and returned (bitsknn_cross_attention_backward); scale as there.
+    workspace: None -> allocated here; or a uint8 device tensor
+    (cross_attention_backward_workspace_bytes).  Returns (grad_queries, grad_keys, grad_values)."""
+    import torch
+    batch, state_heads, states, dim = keys.shape
+    device = queries.device
+    assert queries.is_cuda and keys.shape == values.shape
+    assert queries.shape[0] == batch and queries.shape[3] == dim
+    assert grad_out.shape == queries.shape and out.shape == queries.shape
+    for t in (grad_out, keys, values, out):
+        assert t.dtype == queries.dtype and t.device == device
+    assert lse.dtype == torch.float32 and lse.shape == queries.shape[:3] and lse.is_contiguous()
+    assert lse.device == device
+    grads = []
+    for given, like in ((grad_queries, queries), (grad_keys, keys), (grad_values, values)):
+        given = torch.empty_like(like) if given is None else given
+        assert given.shape == like.shape and given.dtype == like.dtype and given.device == device
+        grads.append(given)
+    shape = _attention_shape(queries, state_heads, states, scale)
+    need = int(lib().bitsknn_cross_attention_backward_workspace_bytes(shape)) if workspace is None else 0
+    workspace, size = _workspace(workspace, need, device)
+    _call(lib().bitsknn_cross_attention_backward, device, shape, _rows(grad_out), _rows(queries), _rows(keys),
+          _rows(values), _rows(out), _ptr(lse), _int32(counts, (batch,), device),
+          *_mask_args(mask, batch, states, device), *(_rows(t) for t in grads), _ptr(workspace), size)
+    return tuple(grads)
+
+
+def cross_attention_backward_workspace_bytes(queries, keys):
+    """What cross_attention_backward wants as a workspace for tensors of these shapes."""
+    return int(lib().bitsknn_cross_attention_backward_workspace_bytes(
         _attention_shape(queries, keys.shape[1], keys.shape[2], 1.0)))
 
 

@@ -431,6 +431,28 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
                             void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Gradients of bitsknn_cross_attention's out with respect to queries, keys and values, from what the
+ * forward call read and returned and the gradient of out (that of lse is taken as zero).  States that
+ * take no part get a gradient of zero; so do rows without any state.  Shared heads' gradients are summed
+ * over the heads that share them; inputs that a stride of 0 repeats get one gradient per repetition
+ * (the gradients' vectors must not overlap).  counts, mask and scale as in the forward call, lse
+ * required.  Every sum has one order: the same call gives the same bits.
+ *   workspace      bitsknn_cross_attention_backward_workspace_bytes bytes, 16-byte aligned; a smaller
+ *                  one is BITSKNN_ERR_INVALID where it does not hold a float per row
+ * Weights and their derivatives are rounded to the vectors' type for the products, sums are fp32 and
+ * the results are rounded once.  Fp16: derivatives of the scores below 2^-24 vanish, so gradients want
+ * a loss scale that keeps them above it.
+ */
+size_t bitsknn_cross_attention_backward_workspace_bytes(const bitsknn_attention_shape* shape);
+int bitsknn_cross_attention_backward(const bitsknn_attention_shape* shape, const bitsknn_rows* grad_out,
+                                     const bitsknn_rows* queries, const bitsknn_rows* keys,
+                                     const bitsknn_rows* values, const bitsknn_rows* out, const float* lse,
+                                     const int32_t* counts, const uint8_t* mask, size_t mask_stride,
+                                     const bitsknn_rows* grad_queries, const bitsknn_rows* grad_keys,
+                                     const bitsknn_rows* grad_values, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/*
  * A cache of states in 8 bits: keys and values as e4m3 codes (OCP: sign, 4 exponent bits, 3 mantissa
  * bits, largest 448) in blocks of `block` states, with one scale for each block and state head; a code
  * stands for its value times the scale.  The caller owns the arrays:

@@ -95,3 +95,49 @@ def made(seed, shape, dtype, spread=1.0):
     gen = torch.Generator()
     gen.manual_seed(seed)
     return (torch.randn(shape, generator=gen) * spread).to(dtype)
+
+
+def gradients(grad_out, queries, keys, values, out, lse, scale, keep):
+    """((grad_queries, its bound), (grad_keys, its bound), (grad_values, its bound)) for the out and lse
+    that are given.
+
+    As above, and: a derivative of a score is P (dP - delta), dP and delta sums of dim products in fp32
+    (off by (dim + 4) e of their absolute sums); it is rounded once to the 16-bit type; the sums over n
+    states or m rows are off by n e, m e of their absolute sums."""
+    dtype = queries.dtype
+    u, tiny = half_step(dtype), least(dtype)
+    b, hs, n, dim = keys.shape
+    share = queries.shape[1] // hs
+    gone = ~keep[:, None, :, None]
+    q, g, o = (x.detach().cpu().double() for x in (queries, grad_out, out))
+    k = keys.detach().cpu().double().masked_fill(gone, 0.0).repeat_interleave(share, 1)
+    v = values.detach().cpu().double().masked_fill(gone, 0.0).repeat_interleave(share, 1)
+    lse = lse.detach().cpu().double()[..., None]
+    lse = lse.masked_fill(lse == -math.inf, math.inf)
+    weights = torch.exp(q @ k.mT * scale - lse).masked_fill(~keep[:, None, None, :], 0.0)
+    size = q.abs() @ k.abs().mT * scale
+    some = lse.abs().masked_fill(lse.isinf(), 0.0)
+    relative = E32 * ((dim + 4) * size + 8 * (size + some) / math.log(2) + 16)
+    delta = (g * o).sum(-1, keepdim=True)
+    change = g @ v.mT - delta
+    change_error = E32 * (dim + 4) * (g.abs() @ v.abs().mT + (g * o).abs().sum(-1, keepdim=True))
+    slope = weights * change
+    slope_error = weights * (relative * change.abs() + change_error) * (1 + u) + (u + 4 * E32) * slope.abs()
+    slope_error = slope_error + tiny * (weights > 0)
+    weight_error = weights * (relative * (1 + u) + u) + tiny * (weights > 0)
+    rows = queries.shape[2] * share
+
+    def shared(x):
+        return x.view(b, hs, share, n, dim).sum(2)
+
+    result = []
+    value = slope @ k * scale
+    bound = scale * (slope_error @ k.abs() + E32 * (n + 4) * (slope.abs() @ k.abs())) + u * value.abs()
+    result.append((value, bound))
+    value = shared(slope.mT @ q) * scale
+    bound = scale * shared(slope_error.mT @ q.abs() + E32 * (rows + 4) * (slope.abs().mT @ q.abs())) + u * value.abs()
+    result.append((value, bound))
+    value = shared(weights.mT @ g)
+    bound = shared(weight_error.mT @ g.abs() + E32 * (rows + 4) * (weights.mT @ g.abs())) + u * value.abs()
+    result.append((value, bound))
+    return [(x, 1.02 * y + 2 * tiny) for x, y in result]
