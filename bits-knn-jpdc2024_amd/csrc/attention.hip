@@ -3,6 +3,8 @@
 #include "attention.hpp"
 
 #include "attention_host.hpp"
+#include "attention_loader.hpp"
+#include "attention_stream.hpp"
 
 namespace bitsknn
 {
@@ -11,96 +13,13 @@ namespace
 
 constexpr u32 TILE_KEYS = 64; // states per tile: the width of a wave's ballot
 constexpr u32 WAVE_ROWS = 32; // rows per wave: the columns of a matrix product
-constexpr u32 WAVES = 4;
 
-// What is known of a tile's states: which take part, and in the cache their scales by sixteens.
-struct tile_states
-{
-    u64 in;
-    float key_scale[4];
-    float value_scale[4];
-};
-
-__device__ __forceinline__ std::int32_t block_of(const attention_args& a, u32 b, u32 j)
-{
-    return a.cache.table[static_cast<std::int64_t>(b) * a.cache.table_stride + (j >> a.cache.block_shift)];
-}
-
-template <bool CACHE>
-__device__ __forceinline__ tile_states look_up(const attention_args& a, u32 b, u32 head, u32 count, u32 first)
-{
-    tile_states t;
-    if constexpr (!CACHE)
-    {
-        t.in = states_taking_part(a, b, count, first);
-    }
-    else
-    {
-        const u32 j = first + (threadIdx.x & 63);
-        bool in = j < count;
-        float ks = 1.0F;
-        float vs = 1.0F;
-        if (in)
-        {
-            const u32 id = static_cast<u32>(block_of(a, b, j));
-            in = id < a.cache.blocks &&
-                 static_cast<std::int32_t>(j & ((1U << a.cache.block_shift) - 1)) < a.cache.block_counts[id];
-            if (in)
-            {
-                const size_t at = static_cast<size_t>(id) * static_cast<u32>(a.state_heads) + head;
-                ks = a.cache.key_scales[at];
-                vs = a.cache.value_scales[at];
-            }
-        }
-        t.in = __ballot(in);
-        // the states of a block that take part are its first ones, so the first of sixteen has the
-        // scale of all that do; where none does, the scale stays 1
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-        {
-            t.key_scale[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 16 * g));
-            t.value_scale[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), 16 * g));
-        }
-    }
-    return t;
-}
-
-// One tile of keys or values into LDS; what takes no part becomes zero.
-template <int DP, typename T, bool CACHE, bool KEYS>
-__device__ __forceinline__ void stage(char* tile, const attention_args& a, u32 b, u32 head, u32 first, u64 in)
-{
-    constexpr u32 CHUNKS = DP / 8;
-    const rows_view& v = KEYS ? a.keys : a.values;
-    const char* base = nullptr;
-    if constexpr (!CACHE)
-    {
-        base = v.data + 2 * (b * v.batch_stride + head * v.head_stride + first * v.row_stride);
-    }
-#pragma unroll
-    for (u32 c = threadIdx.x; c < TILE_KEYS * CHUNKS; c += 64 * WAVES)
-    {
-        const u32 row = c / CHUNKS;
-        const u32 chunk = c % CHUNKS;
-        vuint4 x = {0, 0, 0, 0};
-        if (((in >> row) & 1) != 0 && chunk * 8 < static_cast<u32>(a.dim))
-        {
-            if constexpr (!CACHE)
-            {
-                x = *reinterpret_cast<const vuint4*>(base + 2 * (row * v.row_stride + chunk * 8));
-            }
-            else
-            {
-                const u32 j = first + row;
-                const size_t id = static_cast<u32>(block_of(a, b, j));
-                const size_t at =
-                    (((id * static_cast<u32>(a.state_heads) + head) << a.cache.block_shift) +
-                     (j & ((1U << a.cache.block_shift) - 1))) * static_cast<u32>(a.dim) + chunk * 8;
-                x = decode8<T>(*reinterpret_cast<const vuint2*>((KEYS ? a.cache.key_codes : a.cache.value_codes) + at));
-            }
-        }
-        *reinterpret_cast<vuint4*>(tile + tile_chunk<DP>(row, chunk)) = x;
-    }
-}
+#ifndef TW
+#define TW 8
+#endif
+// Waves that share a tile.  In 256 dimensions a wave needs all the registers of its quarter of the unit.
+constexpr u32 tile_waves(int padded_dim) { return padded_dim <= 128 ? TW : 4; }
+constexpr u32 tile_rows(int padded_dim) { return WAVE_ROWS * tile_waves(padded_dim); }
 
 // What a wave keeps of its 32 rows: lane 32 h + c holds of row c the columns 32 block + 8 (i / 4) +
 // 4 h + i % 4 of the sum.
@@ -177,17 +96,17 @@ __device__ __forceinline__ void store_out(const attention_args& a, const row_sta
     }
 }
 
-// Scores of 32 states (rows of the product) and the wave's 32 rows (columns), weights, and the sum.
+// Bound by the matrix instructions and the LDS reads that feed them.  A workgroup's waves hold 32 rows
+// each and share tiles of 64 states in LDS, two of them: while one is multiplied, the next is on its
+// way into registers and then into the other, so that a step has one barrier.
 template <typename T, int DP, bool CACHE>
-__global__ void __launch_bounds__(64 * WAVES) attention_tile_kernel(const attention_args a)
+__global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attention_tile_kernel(const attention_args a)
 {
-    // the cache's codes are exact in either type; the weights times the values' scale need the range
-    // of bf16, so its second product is taken in bf16 (fp16 queries: the weight as two bf16 pieces,
-    // sixteen bits, so that an fp16 result loses nothing)
-    using V = std::conditional_t<CACHE, __bf16, T>;
-    constexpr bool PIECES = CACHE && std::is_same_v<T, _Float16>;
-    __shared__ __attribute__((aligned(16))) char keys[TILE_KEYS * DP * 2];
-    __shared__ __attribute__((aligned(16))) char values[TILE_KEYS * DP * 2];
+    constexpr u32 THREADS = 64 * tile_waves(DP);
+    using loader = state_loader<T, DP, CACHE, TILE_KEYS, THREADS>;
+    using V = typename loader::V;
+    constexpr u32 TILE_BYTES = TILE_KEYS * DP * 2;
+    __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
     const u32 lane = threadIdx.x & 63;
     const u32 half = lane / 32;
     const u32 id = die_order(blockIdx.x, gridDim.x);
@@ -195,23 +114,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_tile_kernel(const attent
     const u32 split = id / a.row_tiles % a.splits;
     const u32 head = id / a.row_tiles / a.splits % static_cast<u32>(a.state_heads);
     const u32 b = id / a.row_tiles / a.splits / static_cast<u32>(a.state_heads);
-    const u32 row = row_tile * (WAVE_ROWS * WAVES) + threadIdx.x / 64 * WAVE_ROWS + lane % 32;
+    const u32 row = row_tile * tile_rows(DP) + threadIdx.x / 64 * WAVE_ROWS + lane % 32;
 
     vuint4 query[DP / 16];
-    {
-        const u32 r = row < a.rows ? row : 0;
-        const char* q = a.queries.data + 2 * row_offset(a.queries, a, b, head, r);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-        {
-            const u32 at = 16 * s + 8 * half;
-            query[s] = vuint4{0, 0, 0, 0};
-            if (row < a.rows && at < static_cast<u32>(a.dim))
-            {
-                query[s] = *reinterpret_cast<const vuint4*>(q + 2 * at);
-            }
-        }
-    }
+    load_operand<DP>(query, a.queries.data + 2 * row_offset(a.queries, a, b, head, row < a.rows ? row : 0),
+                     row < a.rows, static_cast<u32>(a.dim));
     row_state<DP> st;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
@@ -225,115 +132,157 @@ __global__ void __launch_bounds__(64 * WAVES) attention_tile_kernel(const attent
     const u32 tiles = (count + TILE_KEYS - 1) / TILE_KEYS;
     const u32 begin = static_cast<u32>(static_cast<u64>(tiles) * split / a.splits);
     const u32 end = static_cast<u32>(static_cast<u64>(tiles) * (split + 1) / a.splits);
+    const loader w{a, b, head, count};
+    vuint4 next_keys[loader::LOADS];
+    vuint4 next_values[loader::LOADS];
+    typename loader::place now;   // of the tile in LDS
+    typename loader::place next;  // of the tile in the registers
+    typename loader::place after; // of the tile after it; its table entry is one further ahead
+    u64 in = 0;                   // of the tile in LDS
+    u64 next_in = 0;
+    if (begin < end)
+    {
+        w.look_up_block(now, begin);
+        w.look_up_block(next, begin + 1);
+        w.look_up_block(after, begin + 2);
+        w.look_up_state(now, begin);
+        w.look_up_state(next, begin + 1);
+        in = w.taking_part(now, begin);
+        w.template load<true>(next_keys, now, begin, in);
+        w.template load<false>(next_values, now, begin, in);
+        w.template put<T>(lds, next_keys);
+        w.template put<V>(lds + TILE_BYTES, next_values);
+        __syncthreads();
+    }
     for (u32 tile = begin; tile < end; ++tile)
     {
-        const u32 first = tile * TILE_KEYS;
-        const tile_states t = look_up<CACHE>(a, b, head, count, first);
-        if (t.in == 0)
+        const char* const keys = lds + ((tile - begin) % 2) * 2 * TILE_BYTES;
+        const char* const values = keys + TILE_BYTES;
+        const bool more = tile + 1 < end;
+        const typename loader::place current = now;
+        if (more)
         {
-            continue; // the same in every wave: the workgroup's barriers stay together
+            now = next;
+            next.block = after.block;
+            next_in = w.taking_part(now, tile + 1);
+            w.look_up_block(after, tile + 3);
+            w.look_up_state(next, tile + 2);
+            w.template load<true>(next_keys, now, tile + 1, next_in);
+            w.template load<false>(next_values, now, tile + 1, next_in);
         }
-        __syncthreads();
-        stage<DP, T, CACHE, true>(keys, a, b, head, first, t.in);
-        stage<DP, V, CACHE, false>(values, a, b, head, first, t.in);
-        __syncthreads();
-        vfloat16 score[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
+        if (in != 0) // the same in every wave
         {
-            score[u] = vfloat16{};
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-            {
-                score[u] = mfma<T>::run(tile_row<DP>(keys, 32 * u + lane % 32, s), query[s], score[u]);
-            }
-        }
-        if constexpr (CACHE)
-        {
+            vfloat16 score[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
             {
+                score[u] = vfloat16{};
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+                for (int s = 0; s < DP / 16; ++s)
                 {
-                    score[u][i] *= t.key_scale[2 * u + i / 8];
+                    score[u] = mfma<T>::run(tile_row<DP>(keys, 32 * u + lane % 32, s), query[s], score[u]);
                 }
             }
-        }
-        if (t.in != ~0ULL)
-        {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            if constexpr (CACHE)
             {
-                const u32 bits = static_cast<u32>(t.in >> (32 * u)) >> (4 * half);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+                for (int g = 0; g < 4; ++g)
                 {
-                    score[u][i] = ((bits >> (8 * (i / 4) + i % 4)) & 1) != 0 ? score[u][i] : -__builtin_inff();
+                    const float scale = w.of_sixteen(current.key_scale, g);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        score[g / 2][8 * (g % 2) + i] *= scale;
+                    }
                 }
             }
-        }
-        float top = score[0][0];
+            if (in != ~0ULL)
+            {
 #pragma unroll
-        for (int i = 1; i < 32; ++i)
-        {
-            top = fmaxf(top, score[i / 16][i % 16]);
-        }
-        top = fmaxf(top, other_half(top)) * a.exponent_scale;
-        top = fmaxf(top, st.top);
-        const float base = top == -__builtin_inff() ? 0.0F : top;
-        const float shrink = __builtin_amdgcn_exp2f(st.top - base);
-        st.top = top;
-        float weight = 0.0F;
+                for (int u = 0; u < 2; ++u)
+                {
+                    const u32 bits = static_cast<u32>(in >> (32 * u)) >> (4 * half);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-        {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i / 16][i % 16], a.exponent_scale, -base));
-            score[i / 16][i % 16] = x;
-            weight += x;
-        }
-        st.weight = st.weight * shrink + weight;
+                    for (int i = 0; i < 16; ++i)
+                    {
+                        score[u][i] = ((bits >> (8 * (i / 4) + i % 4)) & 1) != 0 ? score[u][i] : -__builtin_inff();
+                    }
+                }
+            }
+            float most = score[0][0];
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
-        {
-            st.sum[n] *= shrink;
-        }
-        if constexpr (CACHE)
-        {
+            for (int i = 1; i < 32; ++i)
+            {
+                most = fmaxf(most, score[i / 16][i % 16]);
+            }
+            most = fmaxf(most, other_half(most)) * a.exponent_scale;
+            // The reference of the exponents follows the maximum only where that has grown by more than
+            // 8: weights stay below 2^8, and the sums are seldom rescaled.
+            if (__any(most > st.top + 8.0F))
+            {
+                const float top = fmaxf(most, st.top);
+                const float shrink = __builtin_amdgcn_exp2f(st.top - (top == -__builtin_inff() ? 0.0F : top));
+                st.weight *= shrink;
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n)
+                {
+                    st.sum[n] *= shrink;
+                }
+                st.top = top;
+            }
+            const float base = st.top == -__builtin_inff() ? 0.0F : st.top;
+            float weight = 0.0F;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
             {
-                score[i / 16][i % 16] *= t.value_scale[i / 8];
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i / 16][i % 16], a.exponent_scale, -base));
+                score[i / 16][i % 16] = x;
+                weight += x;
+            }
+            st.weight += weight;
+            if constexpr (CACHE)
+            {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                {
+                    // a sixteen without a state that takes part: its weights are zero, its scale may be anything
+                    const float scale = ((in >> (16 * g)) & 0xFFFFU) != 0 ? w.of_sixteen(current.value_scale, g) : 0.0F;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        score[g / 2][8 * (g % 2) + i] *= scale;
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+            {
+                const vuint4 p = operand<V>(score[s / 2], s % 2);
+                vuint4 rest;
+                if constexpr (loader::PIECES)
+                {
+                    rest = operand_rest(score[s / 2], s % 2, p);
+                }
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n)
+                {
+                    const vuint4 v = tile_column<DP>(values, s, n);
+                    st.sum[n] = mfma<V>::run(v, p, st.sum[n]);
+                    if constexpr (loader::PIECES)
+                    {
+                        st.sum[n] = mfma<V>::run(v, rest, st.sum[n]);
+                    }
+                }
             }
         }
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
+        in = next_in;
+        if (more)
         {
-            vuint4 p;
-            vuint4 rest;
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-            {
-                const float x = score[s / 2][8 * (s % 2) + 2 * w];
-                const float y = score[s / 2][8 * (s % 2) + 2 * w + 1];
-                p[w] = pack2<V>(x, y);
-                if constexpr (PIECES)
-                {
-                    rest[w] = pack2<V>(x - __builtin_bit_cast(float, p[w] << 16),
-                                       y - __builtin_bit_cast(float, p[w] & 0xFFFF0000U));
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < DP / 32; ++n)
-            {
-                const vuint4 v = tile_column<DP>(values, s, n);
-                st.sum[n] = mfma<V>::run(v, p, st.sum[n]);
-                if constexpr (PIECES)
-                {
-                    st.sum[n] = mfma<V>::run(v, rest, st.sum[n]);
-                }
-            }
+            char* const other = lds + ((tile + 1 - begin) % 2) * 2 * TILE_BYTES;
+            w.template put<T>(other, next_keys);
+            w.template put<V>(other + TILE_BYTES, next_values);
         }
+        __syncthreads();
     }
     store_rows<DP>(a, st, b, head, row, split);
     if (a.splits == 1)
@@ -409,21 +358,33 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const attention_arg
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
 
-u32 row_tiles_of(size_t rows) { return static_cast<u32>((rows + WAVE_ROWS * WAVES - 1) / (WAVE_ROWS * WAVES)); }
+// Few rows stream past 32 at a time, more of them share tiles of 128 rows.
+constexpr u32 MOST_STREAM_ROWS = 64;
 
-// How many ranges the states are cut into: as many as give the GPU two workgroups per compute unit, at
-// least four tiles each.
+// two per compute unit (1024 and 2048: 3 and 6 us longer for 64 sequences of 32 heads over 8192 states)
+constexpr size_t WANTED_WORKGROUPS = 512;
+
+bool streams(size_t rows) { return rows <= MOST_STREAM_ROWS; }
+
+u32 row_tiles_of(size_t rows, int dim)
+{
+    const size_t per = streams(rows) ? STREAM_ROWS : tile_rows(padded_dim(dim));
+    return static_cast<u32>((rows + per - 1) / per);
+}
+
+// How many ranges the states are cut into: as many as give the GPU enough workgroups, at least 512
+// states each (a join of ranges costs a launch: 12.1 us for three of 333 states, 12.6 us for one of 1000).
 u32 wanted_splits(const bitsknn_attention_shape& s)
 {
     const size_t rows = static_cast<size_t>(s.queries) * static_cast<u32>(s.query_heads / s.state_heads);
-    const size_t groups = static_cast<size_t>(s.batch) * static_cast<u32>(s.state_heads) * row_tiles_of(rows);
-    const size_t tiles = (static_cast<size_t>(s.states) + TILE_KEYS - 1) / TILE_KEYS;
-    if (groups == 0 || groups >= 512)
+    const size_t groups = static_cast<size_t>(s.batch) * static_cast<u32>(s.state_heads) * row_tiles_of(rows, s.dim);
+    const size_t most = static_cast<size_t>(s.states) / 512;
+    if (groups == 0 || groups >= WANTED_WORKGROUPS)
     {
         return 1;
     }
-    size_t splits = (512 + groups - 1) / groups;
-    splits = splits < tiles / 4 ? splits : tiles / 4;
+    size_t splits = (WANTED_WORKGROUPS + groups - 1) / groups;
+    splits = splits < most ? splits : most;
     splits = splits < 64 ? splits : 64;
     return splits < 1 ? 1 : static_cast<u32>(splits);
 }
@@ -448,7 +409,16 @@ int launch(attention_args& a, size_t rows, u32 batch, hipStream_t stream)
     {
         return fail(BITSKNN_ERR_UNSUPPORTED, "attention: too many rows (%zu)", rows);
     }
-    hipLaunchKernelGGL((attention_tile_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)), dim3(64 * WAVES), 0, stream, a);
+    if (streams(a.rows))
+    {
+        hipLaunchKernelGGL((attention_stream_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)),
+                           dim3(64 * STREAM_WAVES), 0, stream, a);
+    }
+    else
+    {
+        hipLaunchKernelGGL((attention_tile_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)), dim3(64 * tile_waves(DP)), 0,
+                           stream, a);
+    }
     BITSKNN_HIP_CHECK(hipGetLastError());
     if (a.splits > 1)
     {
@@ -463,7 +433,7 @@ template <bool CACHE>
 int run(attention_args& a, const bitsknn_attention_shape& s, void* workspace, size_t workspace_bytes, void* stream)
 {
     const size_t rows = static_cast<size_t>(s.batch) * static_cast<u32>(s.query_heads) * static_cast<u32>(s.queries);
-    a.row_tiles = row_tiles_of(a.rows);
+    a.row_tiles = row_tiles_of(a.rows, s.dim);
     a.splits = wanted_splits(s);
     const size_t fit = workspace == nullptr ? 0 : workspace_bytes / bytes_per_split(s);
     if (a.splits > fit)
