@@ -151,15 +151,17 @@ __device__ __forceinline__ float other_half(float x)
 
 // ---- a tile of rows x DP 16-bit values in LDS -------------------------------------------------
 //
-// Rows one after the other in chunks of 16 bytes.  A row's chunks are stored exclusive-or'ed with
-// twice its number modulo eight (in 64 dimensions, where two rows fill the banks, twice half of it):
-// the sixteen-byte reads of eight consecutive rows at one column and the transposed reads of four
-// rows at 32 bytes each then meet every bank once.
+// Rows one after the other in chunks of 16 bytes, a row's chunks stored exclusive-or'ed with a number of
+// the row.  LDS serves 256 bytes at a time, sixteen chunks from different banks, to two kinds of reads:
+// sixteen consecutive rows at one chunk, and (transposed) four rows of which each gives four chunks side
+// by side.  With the row's lowest two bits above its next two, both meet every bank once; in 64
+// dimensions, where two rows fill the banks, the same holds for the bits above the lowest.
+// (Twice the row modulo eight left 44 % of the LDS cycles to conflicts.)
 
 template <int DP>
 __device__ __forceinline__ constexpr u32 tile_swizzle(u32 row)
 {
-    return DP == 64 ? 2 * ((row / 2) % 4) : 2 * (row % 8);
+    return DP == 64 ? 4 * ((row / 2) % 2) + (row / 4) % 4 : 4 * (row % 4) + (row / 4) % 4;
 }
 
 // byte offset of a 16-byte chunk
@@ -187,9 +189,10 @@ __device__ __forceinline__ vuint4 tile_column(const char* tile, u32 step, u32 bl
     const u32 lane = threadIdx.x & 63;
     const u32 row = 16 * step + 4 * (lane / 32) + (lane % 16) / 4;
     const u32 chunk = 4 * block + 2 * ((lane / 16) % 2) + (lane % 4) / 2;
-    const char* at = tile + tile_chunk<DP>(row, chunk) + 8 * (lane % 2);
-    const vshort4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
-    const vshort4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * DP * 2));
+    const char* first = tile + tile_chunk<DP>(row, chunk) + 8 * (lane % 2);
+    const char* second = tile + tile_chunk<DP>(row + 8, chunk) + 8 * (lane % 2);
+    const vshort4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)first);
+    const vshort4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)second);
     const vuint2 lo = __builtin_bit_cast(vuint2, x);
     const vuint2 hi = __builtin_bit_cast(vuint2, y);
     return vuint4{lo.x, lo.y, hi.x, hi.y};
