@@ -11,7 +11,6 @@ namespace bitsknn
 namespace
 {
 
-constexpr u32 TILE_KEYS = 64; // states per tile: the width of a wave's ballot
 constexpr u32 WAVE_ROWS = 32; // rows per wave: the columns of a matrix product
 
 #ifndef TW
@@ -19,6 +18,8 @@ constexpr u32 WAVE_ROWS = 32; // rows per wave: the columns of a matrix product
 #endif
 // Waves that share a tile.  In 256 dimensions a wave needs all the registers of its quarter of the unit.
 constexpr u32 tile_waves(int padded_dim) { return padded_dim <= 128 ? TW : 4; }
+// States per tile: five tiles have to fit LDS.
+constexpr u32 tile_keys(int padded_dim) { return padded_dim <= 128 ? 64 : 32; }
 constexpr u32 tile_rows(int padded_dim) { return WAVE_ROWS * tile_waves(padded_dim); }
 
 // What a wave keeps of its 32 rows: lane 32 h + c holds of row c the columns 32 block + 8 (i / 4) +
@@ -96,17 +97,32 @@ __device__ __forceinline__ void store_out(const attention_args& a, const row_sta
     }
 }
 
-// Bound by the matrix instructions and the LDS reads that feed them.  A workgroup's waves hold 32 rows
-// each and share tiles of 64 states in LDS, two of them: while one is multiplied, the next is on its
-// way into registers and then into the other, so that a step has one barrier.
+// Bound by the matrix instructions.  A workgroup's waves hold 32 rows each and share tiles of states in
+// LDS.  A wave goes through the states by 32: one step takes the scores of the next 32 on the matrix
+// path, turns those of the present 32 into weights on the vector unit meanwhile, multiplies them with
+// the values, and looks for the next scores' maximum.  The next tile's vectors are on their way into
+// registers while a tile is worked on; they are put into LDS (two tiles of keys, three of values, since
+// the slowest wave may still read the last values of the tile before) ahead of a tile's last step, which
+// already reads the next keys: one barrier per tile.
 template <typename T, int DP, bool CACHE>
 __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attention_tile_kernel(const attention_args a)
 {
     constexpr u32 THREADS = 64 * tile_waves(DP);
-    using loader = state_loader<T, DP, CACHE, TILE_KEYS, THREADS>;
+    constexpr u32 KEYS = tile_keys(DP);
+    constexpr u32 STEPS = KEYS / 32;
+    using loader = state_loader<T, DP, CACHE, KEYS, THREADS>;
     using V = typename loader::V;
-    constexpr u32 TILE_BYTES = TILE_KEYS * DP * 2;
-    __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
+    constexpr u32 TILE_BYTES = KEYS * DP * 2;
+    // what a tile's scores need: 0 or -inf to start a score from, and the cache's scales by sixteens
+    struct tile_info
+    {
+        float start[KEYS];
+        float factor[KEYS / 16];
+        float mantissa_log[KEYS / 16];
+        float mantissa_inverse[KEYS / 16];
+    };
+    __shared__ __attribute__((aligned(16))) char lds[5 * TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) tile_info infos[3];
     const u32 lane = threadIdx.x & 63;
     const u32 half = lane / 32;
     const u32 id = die_order(blockIdx.x, gridDim.x);
@@ -127,162 +143,171 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
     }
     st.top = -__builtin_inff();
     st.weight = 0.0F;
+    float base = 0.0F; // top, or 0 while there is none
 
     const u32 count = state_count(a, b);
-    const u32 tiles = (count + TILE_KEYS - 1) / TILE_KEYS;
-    const u32 begin = static_cast<u32>(static_cast<u64>(tiles) * split / a.splits);
-    const u32 end = static_cast<u32>(static_cast<u64>(tiles) * (split + 1) / a.splits);
+    const u32 tiles = (count + KEYS - 1) / KEYS;
+    const u32 begin = uniform(static_cast<u32>(static_cast<u64>(tiles) * split / a.splits));
+    const u32 end = uniform(static_cast<u32>(static_cast<u64>(tiles) * (split + 1) / a.splits));
     const loader w{a, b, head, count};
     vuint4 next_keys[loader::LOADS];
     vuint4 next_values[loader::LOADS];
-    typename loader::place now;   // of the tile in LDS
-    typename loader::place next;  // of the tile in the registers
-    typename loader::place after; // of the tile after it; its table entry is one further ahead
-    u64 in = 0;                   // of the tile in LDS
-    u64 next_in = 0;
+    typename loader::place now;   // of the tile in the registers
+    typename loader::place next;  // of the tile after it
+    typename loader::place after; // its table entry only, one further ahead
+    typename loader::bits in = 0; // of the tile in the registers
+
+    // the tile in the registers into LDS: keys to place k of two, the rest to place v of three
+    const auto put = [&](u32 k, u32 v) {
+        const bool mine = ((in >> (lane % KEYS)) & 1) != 0;
+        const typename loader::scales scales = w.ready(now, mine);
+        w.template put<true>(lds + k * TILE_BYTES, next_keys, 1.0F);
+        w.template put<false>(lds + (2 + v) * TILE_BYTES, next_values, scales.value_scale);
+        if (threadIdx.x < KEYS)
+        {
+            tile_info& t = infos[v];
+            t.start[threadIdx.x] = mine ? 0.0F : -__builtin_inff();
+            if (CACHE && threadIdx.x % 16 == 0)
+            {
+                t.factor[threadIdx.x / 16] = scales.key_factor;
+                t.mantissa_log[threadIdx.x / 16] = scales.mantissa_log;
+                t.mantissa_inverse[threadIdx.x / 16] = scales.mantissa_inverse;
+            }
+        }
+    };
+    // the vectors of tile t on their way into the registers
+    const auto fetch = [&](u32 t) {
+        now = next;
+        next.block = after.block;
+        in = t < end ? w.taking_part(now, t) : 0;
+        w.look_up_block(after, t + 2);
+        w.look_up_state(next, t + 1);
+        w.template load<true>(next_keys, now, t, in);
+        w.template load<false>(next_values, now, t, in);
+    };
+    // scores of the 32 states u of a tile
+    const auto scores_of = [&](u32 k, u32 v, u32 u) {
+        const tile_info& t = infos[v];
+        const char* keys = lds + k * TILE_BYTES;
+        vfloat16 score;
+#pragma unroll
+        for (u32 g = 0; g < 4; ++g)
+        {
+            const vfloat4 start = *reinterpret_cast<const vfloat4*>(t.start + 32 * u + 8 * g + 4 * half);
+#pragma unroll
+            for (u32 i = 0; i < 4; ++i)
+            {
+                score[4 * g + i] = start[i];
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+        {
+            score = mfma<T>::run(tile_row<DP>(keys, 32 * u + lane % 32, s), query[s], score);
+        }
+        return score;
+    };
+    // The reference of the exponents follows the maximum only where that has grown by more than 8:
+    // weights stay below 2^8, and the sums are seldom rescaled.
+    const auto follow = [&](const vfloat16& score, u32 v, u32 u) {
+        const tile_info& t = infos[v];
+        float largest[2] = {score[0], score[8]};
+#pragma unroll
+        for (int i = 1; i < 8; ++i)
+        {
+            largest[0] = fmaxf(largest[0], score[i]);
+            largest[1] = fmaxf(largest[1], score[8 + i]);
+        }
+        float most = CACHE ? fmaxf(largest[0] * t.factor[2 * u], largest[1] * t.factor[2 * u + 1])
+                           : fmaxf(largest[0], largest[1]) * a.exponent_scale;
+        most = fmaxf(most, other_half(most));
+        if (__any(most > st.top + 8.0F))
+        {
+            asm volatile(""); // stays a branch: multiplied every time, the sums cost half the vector work
+            const float from = st.top; // -inf at first: the sums are zero and stay it
+            st.top = fmaxf(most, st.top);
+            base = st.top == -__builtin_inff() ? 0.0F : st.top;
+            const float shrink = __builtin_amdgcn_exp2f(from - base);
+            st.weight *= shrink;
+#pragma unroll
+            for (int n2 = 0; n2 < DP / 32; ++n2)
+            {
+                st.sum[n2] *= shrink;
+            }
+        }
+    };
+
+    vfloat16 score = {};
     if (begin < end)
     {
-        w.look_up_block(now, begin);
-        w.look_up_block(next, begin + 1);
-        w.look_up_block(after, begin + 2);
-        w.look_up_state(now, begin);
-        w.look_up_state(next, begin + 1);
-        in = w.taking_part(now, begin);
-        w.template load<true>(next_keys, now, begin, in);
-        w.template load<false>(next_values, now, begin, in);
-        w.template put<T>(lds, next_keys);
-        w.template put<V>(lds + TILE_BYTES, next_values);
+        w.look_up_block(next, begin);
+        w.look_up_block(after, begin + 1);
+        w.look_up_state(next, begin);
+        fetch(begin);
+        put(0, 0);
+        fetch(begin + 1);
         __syncthreads();
+        score = scores_of(0, 0, 0);
+        follow(score, 0, 0);
     }
+    u32 key_place = 0;
+    u32 value_place = 0;
     for (u32 tile = begin; tile < end; ++tile)
     {
-        const char* const keys = lds + ((tile - begin) % 2) * 2 * TILE_BYTES;
-        const char* const values = keys + TILE_BYTES;
-        const bool more = tile + 1 < end;
-        const typename loader::place current = now;
-        if (more)
+        const u32 next_key_place = 1 - key_place;
+        const u32 next_value_place = value_place == 2 ? 0 : value_place + 1;
+#pragma unroll
+        for (u32 u = 0; u < STEPS; ++u)
         {
-            now = next;
-            next.block = after.block;
-            next_in = w.taking_part(now, tile + 1);
-            w.look_up_block(after, tile + 3);
-            w.look_up_state(next, tile + 2);
-            w.template load<true>(next_keys, now, tile + 1, next_in);
-            w.template load<false>(next_values, now, tile + 1, next_in);
-        }
-        if (in != 0) // the same in every wave
-        {
-            vfloat16 score[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            const bool last = u == STEPS - 1;
+            if (last)
             {
-                score[u] = vfloat16{};
+                put(next_key_place, next_value_place);
+                fetch(tile + 2);
+                __syncthreads();
+            }
+            const tile_info& t = infos[value_place];
+            const char* values = lds + (2 + value_place) * TILE_BYTES;
+            const vfloat16 next_score = last ? scores_of(next_key_place, next_value_place, 0) : scores_of(key_place, value_place, u + 1);
 #pragma unroll
-                for (int s = 0; s < DP / 16; ++s)
+            for (u32 g = 0; g < 2; ++g)
+            {
+                const float factor = CACHE ? t.factor[2 * u + g] : a.exponent_scale;
+                const float from = CACHE ? t.mantissa_log[2 * u + g] - base : -base;
+                float weight = 0.0F;
+#pragma unroll
+                for (u32 i = 8 * g; i < 8 * g + 8; ++i)
                 {
-                    score[u] = mfma<T>::run(tile_row<DP>(keys, 32 * u + lane % 32, s), query[s], score[u]);
+                    score[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], factor, from));
+                    weight += score[i];
                 }
-            }
-            if constexpr (CACHE)
-            {
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                {
-                    const float scale = w.of_sixteen(current.key_scale, g);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                    {
-                        score[g / 2][8 * (g % 2) + i] *= scale;
-                    }
-                }
-            }
-            if (in != ~0ULL)
-            {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                {
-                    const u32 bits = static_cast<u32>(in >> (32 * u)) >> (4 * half);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                    {
-                        score[u][i] = ((bits >> (8 * (i / 4) + i % 4)) & 1) != 0 ? score[u][i] : -__builtin_inff();
-                    }
-                }
-            }
-            float most = score[0][0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i)
-            {
-                most = fmaxf(most, score[i / 16][i % 16]);
-            }
-            most = fmaxf(most, other_half(most)) * a.exponent_scale;
-            // The reference of the exponents follows the maximum only where that has grown by more than
-            // 8: weights stay below 2^8, and the sums are seldom rescaled.
-            if (__any(most > st.top + 8.0F))
-            {
-                const float top = fmaxf(most, st.top);
-                const float shrink = __builtin_amdgcn_exp2f(st.top - (top == -__builtin_inff() ? 0.0F : top));
-                st.weight *= shrink;
-#pragma unroll
-                for (int n = 0; n < DP / 32; ++n)
-                {
-                    st.sum[n] *= shrink;
-                }
-                st.top = top;
-            }
-            const float base = st.top == -__builtin_inff() ? 0.0F : st.top;
-            float weight = 0.0F;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-            {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i / 16][i % 16], a.exponent_scale, -base));
-                score[i / 16][i % 16] = x;
-                weight += x;
-            }
-            st.weight += weight;
-            if constexpr (CACHE)
-            {
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                {
-                    // a sixteen without a state that takes part: its weights are zero, its scale may be anything
-                    const float scale = ((in >> (16 * g)) & 0xFFFFU) != 0 ? w.of_sixteen(current.value_scale, g) : 0.0F;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                    {
-                        score[g / 2][8 * (g % 2) + i] *= scale;
-                    }
-                }
+                st.weight = CACHE ? __builtin_fmaf(weight, t.mantissa_inverse[2 * u + g], st.weight) : st.weight + weight;
             }
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 2; ++s)
             {
-                const vuint4 p = operand<V>(score[s / 2], s % 2);
+                const vuint4 p = operand<V>(score, s);
                 vuint4 rest;
                 if constexpr (loader::PIECES)
                 {
-                    rest = operand_rest(score[s / 2], s % 2, p);
+                    rest = operand_rest<V>(score, s, p);
                 }
 #pragma unroll
-                for (int n = 0; n < DP / 32; ++n)
+                for (int m = 0; m < DP / 32; ++m)
                 {
-                    const vuint4 v = tile_column<DP>(values, s, n);
-                    st.sum[n] = mfma<V>::run(v, p, st.sum[n]);
+                    const vuint4 v = tile_column<DP>(values, 2 * u + s, m);
+                    st.sum[m] = mfma<V>::run(v, p, st.sum[m]);
                     if constexpr (loader::PIECES)
                     {
-                        st.sum[n] = mfma<V>::run(v, rest, st.sum[n]);
+                        st.sum[m] = mfma<V>::run(v, rest, st.sum[m]);
                     }
                 }
             }
+            follow(next_score, last ? next_value_place : value_place, last ? 0 : u + 1);
+            score = next_score;
         }
-        in = next_in;
-        if (more)
-        {
-            char* const other = lds + ((tile + 1 - begin) % 2) * 2 * TILE_BYTES;
-            w.template put<T>(other, next_keys);
-            w.template put<V>(other + TILE_BYTES, next_values);
-        }
-        __syncthreads();
+        key_place = next_key_place;
+        value_place = next_value_place;
     }
     store_rows<DP>(a, st, b, head, row, split);
     if (a.splits == 1)

@@ -102,11 +102,12 @@ struct mfma<__bf16>
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     }
-    // two e4m3 codes (the lower or the upper half of x) as two values: exact
+    // two e4m3 codes (the lower or the upper half of x) as two values, times the power of two of `power`
+    // (its mantissa is ignored): exact
     template <bool UPPER>
-    static __device__ __forceinline__ u32 decode(u32 x)
+    static __device__ __forceinline__ u32 decode(u32 x, float power)
     {
-        return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0F, UPPER));
+        return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, power, UPPER));
     }
 };
 
@@ -120,9 +121,9 @@ struct mfma<_Float16>
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     }
     template <bool UPPER>
-    static __device__ __forceinline__ u32 decode(u32 x)
+    static __device__ __forceinline__ u32 decode(u32 x, float power)
     {
-        return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0F, UPPER));
+        return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, power, UPPER));
     }
 };
 
@@ -133,12 +134,12 @@ __device__ __forceinline__ u32 pack2(float x, float y)
     return __builtin_bit_cast(u32, __builtin_convertvector((vfloat2{x, y}), typename mfma<T>::v2));
 }
 
-// eight e4m3 codes as eight 16-bit values
+// eight e4m3 codes as eight 16-bit values, times the power of two of `power`
 template <typename T>
-__device__ __forceinline__ vuint4 decode8(vuint2 codes)
+__device__ __forceinline__ vuint4 decode8(vuint2 codes, float power)
 {
-    return vuint4{mfma<T>::template decode<false>(codes.x), mfma<T>::template decode<true>(codes.x),
-                  mfma<T>::template decode<false>(codes.y), mfma<T>::template decode<true>(codes.y)};
+    return vuint4{mfma<T>::template decode<false>(codes.x, power), mfma<T>::template decode<true>(codes.x, power),
+                  mfma<T>::template decode<false>(codes.y, power), mfma<T>::template decode<true>(codes.y, power)};
 }
 
 // the value of the lane in the other half of the wave
@@ -198,7 +199,53 @@ __device__ __forceinline__ vuint4 tile_column(const char* tile, u32 step, u32 bl
     return vuint4{lo.x, lo.y, hi.x, hi.y};
 }
 
+// The same reads from addresses that a lane works out once per tile: the steps and the blocks of a tile
+// differ from the first in bits that an exclusive or sets, so one register stands for all of them
+// (tiles that start at multiples of 512 bytes).
+template <typename V>
+__device__ __forceinline__ V lds_read(u32 at)
+{
+    typedef __attribute__((address_space(3))) const V* lds_ptr;
+    return *(lds_ptr)(static_cast<std::uintptr_t>(at));
+}
+
+__device__ __forceinline__ u32 lds_address(const char* p)
+{
+    return static_cast<u32>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// read row `row` at step s: row_address ^ (32 s)
+template <int DP>
+__device__ __forceinline__ u32 row_address(const char* tile, u32 row)
+{
+    return lds_address(tile) + tile_chunk<DP>(row, (threadIdx.x & 63) / 32);
+}
+
+// read the transposed step s at block n: column_address(0) ^ (64 n) and column_address(8) ^ (64 n), both
+// plus 16 s rows
+template <int DP>
+__device__ __forceinline__ u32 column_address(const char* tile, u32 second)
+{
+    const u32 lane = threadIdx.x & 63;
+    const u32 row = 4 * (lane / 32) + (lane % 16) / 4 + second;
+    return lds_address(tile) + tile_chunk<DP>(row, 2 * ((lane / 16) % 2) + (lane % 4) / 2) + 8 * (lane % 2);
+}
+
+__device__ __forceinline__ vuint4 read_column(u32 first, u32 second)
+{
+    typedef __attribute__((address_space(3))) vshort4* lds_ptr;
+    const vuint2 lo = __builtin_bit_cast(vuint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(static_cast<std::uintptr_t>(first))));
+    const vuint2 hi = __builtin_bit_cast(vuint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(static_cast<std::uintptr_t>(second))));
+    return vuint4{lo.x, lo.y, hi.x, hi.y};
+}
+
 // ---- rows and states --------------------------------------------------------------------------
+
+// a value that all lanes hold, in a scalar register
+__device__ __forceinline__ u32 uniform(u32 x)
+{
+    return static_cast<u32>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
 
 // The states [0, count) of sequence b
 __device__ __forceinline__ u32 state_count(const attention_args& a, u32 b)

@@ -9,34 +9,47 @@
 // tiles of rows with those of the queries' gradients: seven products instead of the five of a single
 // walk, and in return no sum is shared between workgroups: every result has one order of addition.
 #include "attention_host.hpp"
+#include "attention_loader.hpp"
 
 namespace bitsknn
 {
 namespace
 {
 
-constexpr u32 WAVES = 4;
-constexpr u32 GRAD_KEYS = 32 * WAVES; // states per workgroup of the walk by states
-constexpr u32 GRAD_ROWS = 32 * WAVES; // rows per workgroup of the walk by rows
-constexpr u32 TILE = 32;              // rows, or states, per step of either walk
+// The walk by rows: four waves of 32 rows each share tiles of states, in 128 dimensions of 32 states (64:
+// 26 registers spilled, 1243 against 957 us for 2 x 16/4 heads, 2048 x 8192).
+constexpr u32 ROW_WAVES = 4;
+constexpr u32 ROW_THREADS = 64 * ROW_WAVES;
+constexpr u32 GRAD_ROWS = 32 * ROW_WAVES;
+constexpr u32 step_keys(int padded_dim) { return padded_dim <= 64 ? 64 : 32; }
 
-// One row of delta per wave.
-template <typename T>
+// The walk by states: waves of 32 states each share steps of 32 rows.  In 128 dimensions a wave keeps its
+// values in LDS instead of in registers, so that two waves per quarter of the unit have room (74
+// registers spilled otherwise), and eight waves share the steps (four: 847 against 791 us).
+constexpr u32 STEP_ROWS = 32;
+constexpr bool values_in_lds(int padded_dim) { return padded_dim == 128; }
+constexpr u32 state_waves(int padded_dim) { return padded_dim == 128 ? 8 : 4; }
+constexpr u32 states_per_group(int padded_dim) { return 32 * state_waves(padded_dim); }
+
+// Both walks take workgroups in the order of their numbers, which deals the tiles of a sequence and head
+// out to all dies: sequences of different lengths then end together (one die per sequence and head: 4 %
+// longer).
+
+// Eight values per lane, DP / 8 lanes per row.
+template <typename T, int DP>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const attention_grad_args g, size_t rows)
 {
     const attention_args& a = g.f;
-    const size_t flat = static_cast<size_t>(blockIdx.x) * 4 + threadIdx.x / 64;
-    const u32 lane = threadIdx.x & 63;
-    if (flat >= rows)
-    {
-        return;
-    }
-    const u32 row = static_cast<u32>(flat % a.rows);
-    const u32 head = static_cast<u32>(flat / a.rows % static_cast<u32>(a.state_heads));
-    const u32 b = static_cast<u32>(flat / a.rows / static_cast<u32>(a.state_heads));
+    constexpr u32 LANES = DP / 8;
+    const size_t flat = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+    const u32 lane = threadIdx.x % LANES;
     float sum = 0.0F;
-    if (8 * lane < static_cast<u32>(a.dim))
+    if (flat < rows && 8 * lane < static_cast<u32>(a.dim))
     {
+        const u32 row = static_cast<u32>(flat % a.rows);
+        const u32 group = static_cast<u32>(flat / a.rows);
+        const u32 head = group % static_cast<u32>(a.state_heads);
+        const u32 b = group / static_cast<u32>(a.state_heads);
         using v8 = typename mfma<T>::v8;
         const v8 x = *reinterpret_cast<const v8*>(a.out.data + 2 * row_offset(a.out, a, b, head, row) + 16 * lane);
         const v8 y = *reinterpret_cast<const v8*>(g.grad_out.data + 2 * row_offset(g.grad_out, a, b, head, row) + 16 * lane);
@@ -47,11 +60,11 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const attention_gr
         }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2)
+    for (u32 o = LANES / 2; o > 0; o /= 2)
     {
-        sum += __shfl_xor(sum, o);
+        sum += __shfl_xor(sum, static_cast<int>(o));
     }
-    if (lane == 0)
+    if (lane == 0 && flat < rows)
     {
         g.delta[flat] = sum;
     }
@@ -63,65 +76,88 @@ __device__ __forceinline__ float exponent_base(float lse)
     return lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
 }
 
-// Two tiles of 32 rows (first of them `first`) of the row views x and y into LDS, and what a row's
-// scores need: the base of its exponents and its delta.  Rows behind the last one are zero with
-// weights of zero.
+// Steps of 32 rows of queries and incoming gradients into LDS, and what a row's scores need: the base of
+// its exponents and its delta.  Rows behind the last one are zero with weights of zero.
 template <int DP>
-__device__ __forceinline__ void stage_rows(char* x_tile, char* y_tile, float* base, float* delta,
-                                           const attention_grad_args& g, u32 b, u32 head, u32 first)
+struct row_loader
 {
-    constexpr u32 CHUNKS = DP / 8;
-    const attention_args& a = g.f;
-#pragma unroll
-    for (u32 c = threadIdx.x; c < TILE * CHUNKS; c += 64 * WAVES)
-    {
-        const u32 row = c / CHUNKS;
-        const u32 chunk = c % CHUNKS;
-        vuint4 x = {0, 0, 0, 0};
-        vuint4 y = {0, 0, 0, 0};
-        if (first + row < a.rows && chunk * 8 < static_cast<u32>(a.dim))
-        {
-            x = *reinterpret_cast<const vuint4*>(a.queries.data + 2 * row_offset(a.queries, a, b, head, first + row) +
-                                                 16 * chunk);
-            y = *reinterpret_cast<const vuint4*>(g.grad_out.data + 2 * row_offset(g.grad_out, a, b, head, first + row) +
-                                                 16 * chunk);
-        }
-        *reinterpret_cast<vuint4*>(x_tile + tile_chunk<DP>(row, chunk)) = x;
-        *reinterpret_cast<vuint4*>(y_tile + tile_chunk<DP>(row, chunk)) = y;
-    }
-    if (threadIdx.x < TILE)
-    {
-        const u32 row = first + threadIdx.x;
-        const size_t flat = (static_cast<size_t>(b) * static_cast<u32>(a.state_heads) + head) * a.rows + row;
-        base[threadIdx.x] = row < a.rows ? exponent_base(a.lse[flat]) : __builtin_inff();
-        delta[threadIdx.x] = row < a.rows ? g.delta[flat] : 0.0F;
-    }
-}
+    static constexpr u32 THREADS = 64 * state_waves(DP);
+    static constexpr u32 CHUNKS = DP / 8;
+    static constexpr int LOADS = STEP_ROWS * CHUNKS / THREADS;
+    static_assert(LOADS >= 1 && STEP_ROWS * CHUNKS % THREADS == 0);
 
-// registers 8 s .. 8 s + 7 of a product as the operand of step s
-template <typename T>
-__device__ __forceinline__ vuint4 operand(const vfloat16& x, int s)
-{
-    return vuint4{pack2<T>(x[8 * s], x[8 * s + 1]), pack2<T>(x[8 * s + 2], x[8 * s + 3]),
-                  pack2<T>(x[8 * s + 4], x[8 * s + 5]), pack2<T>(x[8 * s + 6], x[8 * s + 7])};
-}
+    const attention_grad_args& g;
+    const u32 b;
+    const u32 head;
+    // where the step's first row stands: the same in all lanes, moved on by 32 rows per step
+    u32 first = 0;
+    u32 first_in_group = 0;
+    u32 first_position = 0;
+    vuint4 queries[LOADS];
+    vuint4 grads[LOADS];
+    float lse;
+    float delta;
 
-// one of 32 consecutive vectors in the operand layout of its lane
-template <int DP>
-__device__ __forceinline__ void load_vector(vuint4 (&x)[DP / 16], const char* at, bool in, u32 dim)
-{
-    const u32 half = (threadIdx.x & 63) / 32;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s)
+    __device__ __forceinline__ void fetch()
     {
-        const u32 column = 16 * s + 8 * half;
-        x[s] = vuint4{0, 0, 0, 0};
-        if (in && column < dim)
+        const attention_args& a = g.f;
+        const u32 chunk = threadIdx.x % CHUNKS;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
         {
-            x[s] = *reinterpret_cast<const vuint4*>(at + 2 * column);
+            const u32 row = (static_cast<u32>(i) * THREADS + threadIdx.x) / CHUNKS;
+            u32 in_group = first_in_group;
+            u32 position = first_position + row;
+            while (position >= a.queries_per_head)
+            {
+                position -= a.queries_per_head;
+                ++in_group;
+            }
+            queries[i] = vuint4{0, 0, 0, 0};
+            grads[i] = vuint4{0, 0, 0, 0};
+            if (first + row < a.rows && chunk * 8 < static_cast<u32>(a.dim))
+            {
+                const u32 h = head * static_cast<u32>(a.group) + in_group;
+                queries[i] = *reinterpret_cast<const vuint4*>(
+                    a.queries.data + 2 * (b * a.queries.batch_stride + h * a.queries.head_stride + position * a.queries.row_stride) + 16 * chunk);
+                grads[i] = *reinterpret_cast<const vuint4*>(
+                    g.grad_out.data + 2 * (b * g.grad_out.batch_stride + h * g.grad_out.head_stride + position * g.grad_out.row_stride) + 16 * chunk);
+            }
+        }
+        lse = __builtin_inff();
+        delta = 0.0F;
+        if (threadIdx.x < STEP_ROWS && first + threadIdx.x < a.rows)
+        {
+            const size_t flat = (static_cast<size_t>(b) * static_cast<u32>(a.state_heads) + head) * a.rows + first + threadIdx.x;
+            lse = a.lse[flat];
+            delta = g.delta[flat];
+        }
+        first += STEP_ROWS;
+        first_position += STEP_ROWS;
+        while (first_position >= a.queries_per_head)
+        {
+            first_position -= a.queries_per_head;
+            ++first_in_group;
         }
     }
-}
+
+    __device__ __forceinline__ void put(char* query_tile, char* grad_tile, float* bases, float* deltas) const
+    {
+        const u32 chunk = threadIdx.x % CHUNKS;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const u32 at = tile_chunk<DP>((static_cast<u32>(i) * THREADS + threadIdx.x) / CHUNKS, chunk);
+            *reinterpret_cast<vuint4*>(query_tile + at) = queries[i];
+            *reinterpret_cast<vuint4*>(grad_tile + at) = grads[i];
+        }
+        if (threadIdx.x < STEP_ROWS)
+        {
+            bases[threadIdx.x] = exponent_base(lse);
+            deltas[threadIdx.x] = delta;
+        }
+    }
+};
 
 // a lane's column of a transposed sum (dim x 32), times a factor
 template <typename T, int DP>
@@ -146,22 +182,25 @@ __device__ __forceinline__ void store_vector(char* at, const vfloat16 (&x)[DP / 
 }
 
 // By states: a wave keeps 32 keys and values as operands and their gradients' sums, and walks over the
-// rows that read them, those of all heads that share them.
+// rows that read them, those of all heads that share them.  While 32 rows are multiplied, the next are on
+// their way into registers and then into the other half of LDS: one barrier per step.
 template <typename T, int DP>
-__global__ void __launch_bounds__(64 * WAVES) attention_grad_states_kernel(const attention_grad_args g)
+__global__ void __launch_bounds__(64 * state_waves(DP), DP <= 128 ? 2 : 1) attention_grad_states_kernel(const attention_grad_args g)
 {
     const attention_args& a = g.f;
-    __shared__ __attribute__((aligned(16))) char query_tile[TILE * DP * 2];
-    __shared__ __attribute__((aligned(16))) char grad_tile[TILE * DP * 2];
-    __shared__ __attribute__((aligned(16))) float base[TILE];
-    __shared__ __attribute__((aligned(16))) float delta[TILE];
+    constexpr u32 TILE_BYTES = STEP_ROWS * DP * 2;
+    constexpr bool KEEP = !values_in_lds(DP);
+    __shared__ __attribute__((aligned(512))) char lds[4 * TILE_BYTES];
+    __shared__ __attribute__((aligned(512))) char kept[KEEP ? 16 : states_per_group(DP) * DP * 2];
+    __shared__ __attribute__((aligned(16))) float bases[2][STEP_ROWS];
+    __shared__ __attribute__((aligned(16))) float deltas[2][STEP_ROWS];
     const u32 lane = threadIdx.x & 63;
     const u32 half = lane / 32;
-    const u32 id = die_order(blockIdx.x, gridDim.x);
+    const u32 id = blockIdx.x;
     const u32 key_tile = id % g.key_tiles;
     const u32 head = id / g.key_tiles % static_cast<u32>(a.state_heads);
     const u32 b = id / g.key_tiles / static_cast<u32>(a.state_heads);
-    const u32 state = key_tile * GRAD_KEYS + threadIdx.x / 64 * 32 + lane % 32;
+    const u32 state = key_tile * states_per_group(DP) + threadIdx.x / 64 * 32 + lane % 32;
     const u32 count = state_count(a, b);
     bool in = state < count;
     if (a.mask != nullptr && in)
@@ -170,10 +209,20 @@ __global__ void __launch_bounds__(64 * WAVES) attention_grad_states_kernel(const
     }
     vuint4 key[DP / 16];
     vuint4 value[DP / 16];
-    load_vector<DP>(key, a.keys.data + 2 * (b * a.keys.batch_stride + head * a.keys.head_stride + state * a.keys.row_stride),
-                    in, static_cast<u32>(a.dim));
-    load_vector<DP>(value, a.values.data + 2 * (b * a.values.batch_stride + head * a.values.head_stride + state * a.values.row_stride),
-                    in, static_cast<u32>(a.dim));
+    load_operand<DP>(key, a.keys.data + 2 * (b * a.keys.batch_stride + head * a.keys.head_stride + state * a.keys.row_stride),
+                     in, static_cast<u32>(a.dim));
+    load_operand<DP>(value, a.values.data + 2 * (b * a.values.batch_stride + head * a.values.head_stride + state * a.values.row_stride),
+                     in, static_cast<u32>(a.dim));
+    char* const my_values = kept + (KEEP ? 0 : threadIdx.x / 64 * 32 * DP * 2);
+    if constexpr (!KEEP)
+    {
+        // a wave's own part: no barrier
+#pragma unroll
+        for (u32 s = 0; s < DP / 16; ++s)
+        {
+            *reinterpret_cast<vuint4*>(my_values + tile_chunk<DP>(lane % 32, 2 * s + half)) = value[s];
+        }
+    }
     vfloat16 key_sum[DP / 32];
     vfloat16 value_sum[DP / 32];
 #pragma unroll
@@ -182,48 +231,71 @@ __global__ void __launch_bounds__(64 * WAVES) attention_grad_states_kernel(const
         key_sum[n] = vfloat16{};
         value_sum[n] = vfloat16{};
     }
-    const u32 steps = __syncthreads_or(in) != 0 ? (a.rows + TILE - 1) / TILE : 0;
-    for (u32 step = 0; step < steps; ++step)
+    const u32 steps = __syncthreads_or(in) != 0 ? (a.rows + STEP_ROWS - 1) / STEP_ROWS : 0;
+    if (steps > 0)
     {
+        row_loader<DP> rows{g, b, head};
+        rows.fetch();
+        rows.put(lds, lds + TILE_BYTES, bases[0], deltas[0]);
         __syncthreads();
-        stage_rows<DP>(query_tile, grad_tile, base, delta, g, b, head, step * TILE);
-        __syncthreads();
-        vfloat16 p = {};
-        vfloat16 slope = {};
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        const u32 row_at = row_address<DP>(lds, lane % 32);
+        const u32 value_at = row_address<DP>(my_values, lane % 32);
+        const u32 first_at = column_address<DP>(lds, 0);
+        const u32 second_at = column_address<DP>(lds, 8);
+        for (u32 step = 0; step < steps; ++step)
         {
-            p = mfma<T>::run(tile_row<DP>(query_tile, lane % 32, s), key[s], p);
-        }
+            const u32 place = step % 2;
+            // hidden from the compiler, which would keep the addresses of every step and block in
+            // registers that the sums need
+            u32 row = row_at + place * 2 * TILE_BYTES;
+            u32 own = value_at;
+            u32 first = first_at + place * 2 * TILE_BYTES;
+            u32 second = second_at + place * 2 * TILE_BYTES;
+            asm volatile("" : "+v"(row), "+v"(own), "+v"(first), "+v"(second));
+            rows.fetch();
+            vfloat16 p = {};
+            vfloat16 slope = {};
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-        {
-            slope = mfma<T>::run(tile_row<DP>(grad_tile, lane % 32, s), value[s], slope);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-        {
-            const vfloat4 top = *reinterpret_cast<const vfloat4*>(base + 2 * i + 4 * half);
-            const vfloat4 d = *reinterpret_cast<const vfloat4*>(delta + 2 * i + 4 * half);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (u32 s = 0; s < DP / 16; ++s)
             {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i + j], a.exponent_scale, -top[j]));
-                p[i + j] = x;
-                slope[i + j] = x * (slope[i + j] - d[j]);
+                p = mfma<T>::run(lds_read<vuint4>(row ^ (32 * s)), key[s], p);
             }
-        }
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-        {
-            const vuint4 weight = operand<T>(p, s);
-            const vuint4 change = operand<T>(slope, s);
-#pragma unroll
-            for (int n = 0; n < DP / 32; ++n)
+            for (u32 s = 0; s < DP / 16; ++s)
             {
-                value_sum[n] = mfma<T>::run(tile_column<DP>(grad_tile, s, n), weight, value_sum[n]);
-                key_sum[n] = mfma<T>::run(tile_column<DP>(query_tile, s, n), change, key_sum[n]);
+                const vuint4 v = KEEP ? value[s] : lds_read<vuint4>(own ^ (32 * s));
+                slope = mfma<T>::run(lds_read<vuint4>((row ^ (32 * s)) + TILE_BYTES), v, slope);
             }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+            {
+                const vfloat4 top = *reinterpret_cast<const vfloat4*>(bases[place] + 2 * i + 4 * half);
+                const vfloat4 d = *reinterpret_cast<const vfloat4*>(deltas[place] + 2 * i + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i + j], a.exponent_scale, -top[j]));
+                    p[i + j] = x;
+                    slope[i + j] = x * (slope[i + j] - d[j]);
+                }
+            }
+            const vuint4 weight[2] = {operand<T>(p, 0), operand<T>(p, 1)};
+            const vuint4 change[2] = {operand<T>(slope, 0), operand<T>(slope, 1)};
+#pragma unroll
+            for (u32 n = 0; n < DP / 32; ++n)
+            {
+#pragma unroll
+                for (u32 s = 0; s < 2; ++s)
+                {
+                    const u32 x = (first ^ (64 * n)) + 16 * s * DP * 2;
+                    const u32 y = (second ^ (64 * n)) + 16 * s * DP * 2;
+                    value_sum[n] = mfma<T>::run(read_column(x + TILE_BYTES, y + TILE_BYTES), weight[s], value_sum[n]);
+                    key_sum[n] = mfma<T>::run(read_column(x, y), change[s], key_sum[n]);
+                }
+            }
+            char* const other = lds + (1 - place) * 2 * TILE_BYTES;
+            rows.put(other, other + TILE_BYTES, bases[1 - place], deltas[1 - place]);
+            __syncthreads();
         }
     }
     if (state >= a.states)
@@ -247,99 +319,132 @@ __global__ void __launch_bounds__(64 * WAVES) attention_grad_states_kernel(const
 }
 
 // By rows: a wave keeps 32 rows of queries and incoming gradients as operands and the sums of the
-// queries' gradients, and walks over the states.
+// queries' gradients, and walks over the states, staged as above.  A score starts from 0, or from -inf
+// where the state takes no part: its weight is then 0.
+// The derivatives of a row's scores sum to zero, so what the keys have in common cancels in their
+// product, but not in the rounding errors of the derivatives: they enter in two pieces (3 % more time for
+// 2 x 16/4 heads, 2048 x 8192 x 128; the gradient's error 2.6e-3 -> 1.7e-3, which is its own rounding).
 template <typename T, int DP>
-__global__ void __launch_bounds__(64 * WAVES) attention_grad_rows_kernel(const attention_grad_args g)
+__global__ void __launch_bounds__(ROW_THREADS, DP <= 128 ? 2 : 1) attention_grad_rows_kernel(const attention_grad_args g)
 {
     const attention_args& a = g.f;
-    constexpr u32 CHUNKS = DP / 8;
-    __shared__ __attribute__((aligned(16))) char key_tile[TILE * DP * 2];
-    __shared__ __attribute__((aligned(16))) char value_tile[TILE * DP * 2];
+    constexpr u32 KEYS = step_keys(DP);
+    using loader = state_loader<T, DP, false, KEYS, ROW_THREADS>;
+    constexpr u32 TILE_BYTES = KEYS * DP * 2;
+    __shared__ __attribute__((aligned(512))) char lds[4 * TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) float starts[2][KEYS];
     const u32 lane = threadIdx.x & 63;
     const u32 half = lane / 32;
-    const u32 id = die_order(blockIdx.x, gridDim.x);
+    const u32 id = blockIdx.x;
     const u32 row_tile = id % a.row_tiles;
     const u32 head = id / a.row_tiles % static_cast<u32>(a.state_heads);
     const u32 b = id / a.row_tiles / static_cast<u32>(a.state_heads);
     const u32 row = row_tile * GRAD_ROWS + threadIdx.x / 64 * 32 + lane % 32;
-    const bool in = row < a.rows;
-    const u32 r = in ? row : 0;
+    const bool mine = row < a.rows;
+    const u32 r = mine ? row : 0;
     vuint4 query[DP / 16];
     vuint4 grad[DP / 16];
-    load_vector<DP>(query, a.queries.data + 2 * row_offset(a.queries, a, b, head, r), in, static_cast<u32>(a.dim));
-    load_vector<DP>(grad, g.grad_out.data + 2 * row_offset(g.grad_out, a, b, head, r), in, static_cast<u32>(a.dim));
+    load_operand<DP>(query, a.queries.data + 2 * row_offset(a.queries, a, b, head, r), mine, static_cast<u32>(a.dim));
+    load_operand<DP>(grad, g.grad_out.data + 2 * row_offset(g.grad_out, a, b, head, r), mine, static_cast<u32>(a.dim));
     const size_t flat = (static_cast<size_t>(b) * static_cast<u32>(a.state_heads) + head) * a.rows + r;
-    const float top = in ? exponent_base(a.lse[flat]) : __builtin_inff();
-    const float delta = in ? g.delta[flat] : 0.0F;
+    const float top = mine ? exponent_base(a.lse[flat]) : __builtin_inff();
+    const float delta = mine ? g.delta[flat] : 0.0F;
     vfloat16 sum[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
     {
         sum[n] = vfloat16{};
     }
-    const u32 count = state_count(a, b);
-    for (u32 first = 0; first < count; first += TILE)
+    const u32 count = uniform(state_count(a, b));
+    const u32 tiles = (count + KEYS - 1) / KEYS;
+    const loader w{a, b, head, count};
+    vuint4 keys[loader::LOADS];
+    vuint4 values[loader::LOADS];
+    typename loader::place next;
+    typename loader::bits in = 0; // of the tile in the registers
+    const auto fetch = [&](u32 t) {
+        in = t < tiles ? w.taking_part(next, t) : 0;
+        w.template load<true>(keys, next, t, in);
+        w.template load<false>(values, next, t, in);
+        w.look_up_state(next, t + 1);
+    };
+    const auto put = [&](u32 place) {
+        w.template put<true>(lds + place * 2 * TILE_BYTES, keys, 1.0F);
+        w.template put<false>(lds + place * 2 * TILE_BYTES + TILE_BYTES, values, 1.0F);
+        if (threadIdx.x < KEYS)
+        {
+            starts[place][threadIdx.x] = ((in >> threadIdx.x) & 1) != 0 ? 0.0F : -__builtin_inff();
+        }
+    };
+    if (tiles > 0)
     {
-        const u32 taking = static_cast<u32>(states_taking_part(a, b, count, first));
-        if (taking == 0)
-        {
-            continue;
-        }
+        w.look_up_state(next, 0);
+        fetch(0);
+        put(0);
         __syncthreads();
-        const char* keys = a.keys.data + 2 * (b * a.keys.batch_stride + head * a.keys.head_stride + first * a.keys.row_stride);
-        const char* values = a.values.data + 2 * (b * a.values.batch_stride + head * a.values.head_stride + first * a.values.row_stride);
-#pragma unroll
-        for (u32 c = threadIdx.x; c < TILE * CHUNKS; c += 64 * WAVES)
-        {
-            const u32 j = c / CHUNKS;
-            const u32 chunk = c % CHUNKS;
-            vuint4 x = {0, 0, 0, 0};
-            vuint4 y = {0, 0, 0, 0};
-            if (((taking >> j) & 1) != 0 && chunk * 8 < static_cast<u32>(a.dim))
-            {
-                x = *reinterpret_cast<const vuint4*>(keys + 2 * (j * a.keys.row_stride + chunk * 8));
-                y = *reinterpret_cast<const vuint4*>(values + 2 * (j * a.values.row_stride + chunk * 8));
-            }
-            *reinterpret_cast<vuint4*>(key_tile + tile_chunk<DP>(j, chunk)) = x;
-            *reinterpret_cast<vuint4*>(value_tile + tile_chunk<DP>(j, chunk)) = y;
-        }
-        __syncthreads();
-        vfloat16 p = {};
-        vfloat16 slope = {};
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-        {
-            p = mfma<T>::run(tile_row<DP>(key_tile, lane % 32, s), query[s], p);
-        }
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-        {
-            slope = mfma<T>::run(tile_row<DP>(value_tile, lane % 32, s), grad[s], slope);
-        }
-        const u32 bits = taking >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-        {
-            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.exponent_scale, -top)) * (slope[i] - delta);
-            if (taking != ~0U)
-            {
-                // a state that takes no part was staged as zero; its weight may be infinite
-                x = ((bits >> (8 * (i / 4) + i % 4)) & 1) != 0 ? x : 0.0F;
-            }
-            p[i] = x;
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-        {
-            const vuint4 change = operand<T>(p, s);
-#pragma unroll
-            for (int n = 0; n < DP / 32; ++n)
-            {
-                sum[n] = mfma<T>::run(tile_column<DP>(key_tile, s, n), change, sum[n]);
-            }
-        }
     }
-    if (in)
+    const u32 row_at = row_address<DP>(lds, lane % 32);
+    const u32 first_at = column_address<DP>(lds, 0);
+    const u32 second_at = column_address<DP>(lds, 8);
+    for (u32 tile = 0; tile < tiles; ++tile)
+    {
+        const u32 place = tile % 2;
+        fetch(tile + 1);
+#pragma unroll 1
+        for (u32 u = 0; u < KEYS / 32; ++u)
+        {
+            const u32 at = place * 2 * TILE_BYTES + u * 32 * DP * 2;
+            u32 row_to = row_at + at;
+            u32 first = first_at + at;
+            u32 second = second_at + at;
+            // hidden from the compiler, as in the walk by states
+            asm volatile("" : "+v"(row_to), "+v"(first), "+v"(second));
+            vfloat16 p;
+            vfloat16 slope = {};
+#pragma unroll
+            for (u32 q = 0; q < 4; ++q)
+            {
+                const vfloat4 start = *reinterpret_cast<const vfloat4*>(starts[place] + 32 * u + 8 * q + 4 * half);
+#pragma unroll
+                for (u32 i = 0; i < 4; ++i)
+                {
+                    p[4 * q + i] = start[i];
+                }
+            }
+#pragma unroll
+            for (u32 s = 0; s < DP / 16; ++s)
+            {
+                p = mfma<T>::run(lds_read<vuint4>(row_to ^ (32 * s)), query[s], p);
+            }
+#pragma unroll
+            for (u32 s = 0; s < DP / 16; ++s)
+            {
+                slope = mfma<T>::run(lds_read<vuint4>((row_to ^ (32 * s)) + TILE_BYTES), grad[s], slope);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.exponent_scale, -top)) * (slope[i] - delta);
+            }
+            const vuint4 change[2] = {operand<T>(p, 0), operand<T>(p, 1)};
+            const vuint4 rest[2] = {operand_rest<T>(p, 0, change[0]), operand_rest<T>(p, 1, change[1])};
+#pragma unroll
+            for (u32 n = 0; n < DP / 32; ++n)
+            {
+#pragma unroll
+                for (u32 s = 0; s < 2; ++s)
+                {
+                    const u32 rows_on = 16 * s * DP * 2;
+                    const vuint4 k = read_column((first ^ (64 * n)) + rows_on, (second ^ (64 * n)) + rows_on);
+                    sum[n] = mfma<T>::run(k, change[s], sum[n]);
+                    sum[n] = mfma<T>::run(k, rest[s], sum[n]);
+                }
+            }
+        }
+        put(1 - place);
+        __syncthreads();
+    }
+    if (mine)
     {
         store_vector<T, DP>(g.grad_queries.data + 2 * row_offset(g.grad_queries, a, b, head, row), sum, a.scale,
                             static_cast<u32>(a.dim));
@@ -352,16 +457,18 @@ int launch(const attention_grad_args& g, size_t rows, u32 batch, hipStream_t str
     const u64 groups = static_cast<u64>(batch) * static_cast<u32>(g.f.state_heads);
     if (rows > 0)
     {
-        hipLaunchKernelGGL(attention_delta_kernel<T>, dim3(static_cast<u32>((rows + 3) / 4)), dim3(256), 0, stream, g, rows);
+        constexpr size_t per_group = 256 / (DP / 8);
+        hipLaunchKernelGGL((attention_delta_kernel<T, DP>), dim3(static_cast<u32>((rows + per_group - 1) / per_group)),
+                           dim3(256), 0, stream, g, rows);
         BITSKNN_HIP_CHECK(hipGetLastError());
         hipLaunchKernelGGL((attention_grad_rows_kernel<T, DP>), dim3(static_cast<u32>(groups * g.f.row_tiles)),
-                           dim3(64 * WAVES), 0, stream, g);
+                           dim3(ROW_THREADS), 0, stream, g);
         BITSKNN_HIP_CHECK(hipGetLastError());
     }
     if (g.f.states > 0)
     {
         hipLaunchKernelGGL((attention_grad_states_kernel<T, DP>), dim3(static_cast<u32>(groups * g.key_tiles)),
-                           dim3(64 * WAVES), 0, stream, g);
+                           dim3(64 * state_waves(DP)), 0, stream, g);
         BITSKNN_HIP_CHECK(hipGetLastError());
     }
     return BITSKNN_OK;
@@ -436,8 +543,9 @@ extern "C" int bitsknn_cross_attention_backward(const bitsknn_attention_shape* s
         return fail(BITSKNN_ERR_INVALID, "%s: a workspace of %zu bytes, %zu are needed", name,
                     workspace == nullptr ? size_t{0} : workspace_bytes, need);
     }
+    const int padded = s.dim <= 64 ? 64 : (s.dim <= 128 ? 128 : 256);
     a.row_tiles = (a.rows + GRAD_ROWS - 1) / GRAD_ROWS;
-    g.key_tiles = (a.states + GRAD_KEYS - 1) / GRAD_KEYS;
+    g.key_tiles = (a.states + states_per_group(padded) - 1) / states_per_group(padded);
     const u64 groups = static_cast<u64>(s.batch) * static_cast<u32>(hs);
     if (groups * a.row_tiles > MOST_WORKGROUPS || groups * g.key_tiles > MOST_WORKGROUPS ||
         (rows + 3) / 4 > MOST_WORKGROUPS)
@@ -449,7 +557,6 @@ extern "C" int bitsknn_cross_attention_backward(const bitsknn_attention_shape* s
     a.mask_stride = static_cast<std::int64_t>(mask_stride);
     a.lse = const_cast<float*>(lse);
     g.delta = static_cast<float*>(workspace);
-    const int padded = s.dim <= 64 ? 64 : (s.dim <= 128 ? 128 : 256);
     const auto st = static_cast<hipStream_t>(stream);
     const u32 batch = static_cast<u32>(s.batch);
     if (s.type == BITSKNN_BF16)

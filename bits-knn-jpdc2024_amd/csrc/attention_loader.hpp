@@ -22,9 +22,9 @@ struct state_loader
     static constexpr bool SPARE = KEYS * CHUNKS < THREADS; // more threads than loads
     static constexpr int LOADS = SPARE ? 1 : KEYS * CHUNKS / THREADS; // per thread and matrix
     static constexpr int SIXTEENS = KEYS / 16;
-    // the cache's codes are exact in either type; a weight times its values' scale needs the range of
-    // bf16, so the second product is taken in bf16 (fp16 queries: the weight as two bf16 pieces,
-    // sixteen bits, so that an fp16 result loses nothing)
+    // the cache's keys are exact in either type; its values times their scale need the range of bf16, so
+    // the second product is taken in bf16 (fp16 queries: a weight as two bf16 pieces, sixteen bits, so
+    // that an fp16 result loses nothing)
     using V = std::conditional_t<CACHE, __bf16, T>;
     static constexpr bool PIECES = CACHE && std::is_same_v<T, _Float16>;
     using bits = std::conditional_t<KEYS == 64, u64, u32>;
@@ -35,6 +35,14 @@ struct state_loader
         std::int32_t held = 0;  // states in the block (cache); mask byte
         float key_scale = 1.0F;
         float value_scale = 1.0F;
+    };
+
+    struct scales
+    {
+        float key_factor = 1.0F;
+        float value_scale = 1.0F; // its power of two counts
+        float mantissa_log = 0.0F;
+        float mantissa_inverse = 1.0F;
     };
 
     const attention_args& a;
@@ -104,6 +112,28 @@ struct state_loader
         return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 16 * g));
     }
 
+    // A lane's scales, ready for use.  States that take part are a block's first ones, so the first of a
+    // sixteen has the scales of all that do; where it takes no part they are 1.  A key's scale
+    // multiplies the factor from scores to exponents (at least the least normal number: a masked score
+    // of -inf stays one).  Of a value's scale the power of two goes into the decoded values, exactly
+    // (bf16 has the exponents), and the mantissa into the exponents of the weights; the sum of weights
+    // takes it out again.
+    __device__ __forceinline__ scales ready(const place& p, bool in) const
+    {
+        scales s;
+        if constexpr (CACHE)
+        {
+            const float key = in ? p.key_scale * a.exponent_scale : 1.0F;
+            s.key_factor = key < 1.17549435e-38F ? 1.17549435e-38F : key;
+            s.value_scale = in ? p.value_scale : 1.0F;
+            const float mantissa =
+                __builtin_bit_cast(float, (__builtin_bit_cast(u32, s.value_scale) & 0x007FFFFFU) | 0x3F800000U);
+            s.mantissa_log = __builtin_amdgcn_logf(mantissa);
+            s.mantissa_inverse = __builtin_amdgcn_rcpf(mantissa);
+        }
+        return s;
+    }
+
     // The tile's vectors into registers: neighbouring threads take neighbouring chunks of a row.  What
     // takes no part is zero.
     template <bool KEY>
@@ -170,9 +200,10 @@ struct state_loader
         }
     }
 
-    template <typename E>
-    __device__ __forceinline__ void put(char* tile, const vuint4 (&x)[LOADS]) const
+    template <bool KEY>
+    __device__ __forceinline__ void put(char* tile, const vuint4 (&x)[LOADS], float scale) const
     {
+        using E = std::conditional_t<KEY, T, V>;
         const u32 t = threadIdx.x % THREADS;
         const u32 chunk = t % CHUNKS;
 #pragma unroll
@@ -185,8 +216,13 @@ struct state_loader
             }
             if constexpr (CACHE)
             {
-                *reinterpret_cast<vuint4*>(tile + tile_chunk<DP>(row, 2 * chunk)) = decode8<E>(vuint2{x[i].x, x[i].y});
-                *reinterpret_cast<vuint4*>(tile + tile_chunk<DP>(row, 2 * chunk + 1)) = decode8<E>(vuint2{x[i].z, x[i].w});
+                float power = 1.0F;
+                if constexpr (!KEY)
+                {
+                    power = of_sixteen(scale, __builtin_amdgcn_readfirstlane(static_cast<int>(row / 16)) % SIXTEENS);
+                }
+                *reinterpret_cast<vuint4*>(tile + tile_chunk<DP>(row, 2 * chunk)) = decode8<E>(vuint2{x[i].x, x[i].y}, power);
+                *reinterpret_cast<vuint4*>(tile + tile_chunk<DP>(row, 2 * chunk + 1)) = decode8<E>(vuint2{x[i].z, x[i].w}, power);
             }
             else
             {
@@ -221,15 +257,28 @@ __device__ __forceinline__ vuint4 operand(const vfloat16& x, int s)
                   pack2<V>(x[8 * s + 4], x[8 * s + 5]), pack2<V>(x[8 * s + 6], x[8 * s + 7])};
 }
 
-// what bf16 operand `p` leaves of its values
+// what operand `p` leaves of its values, as an operand of its own
+template <typename V>
 __device__ __forceinline__ vuint4 operand_rest(const vfloat16& x, int s, vuint4 p)
 {
     vuint4 rest;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
     {
-        rest[k] = pack2<__bf16>(x[8 * s + 2 * k] - __builtin_bit_cast(float, p[k] << 16),
-                                x[8 * s + 2 * k + 1] - __builtin_bit_cast(float, p[k] & 0xFFFF0000U));
+        float lo;
+        float hi;
+        if constexpr (std::is_same_v<V, __bf16>)
+        {
+            lo = __builtin_bit_cast(float, p[k] << 16);
+            hi = __builtin_bit_cast(float, p[k] & 0xFFFF0000U);
+        }
+        else
+        {
+            const auto both = __builtin_bit_cast(typename mfma<V>::v2, p[k]);
+            lo = static_cast<float>(both[0]);
+            hi = static_cast<float>(both[1]);
+        }
+        rest[k] = pack2<V>(x[8 * s + 2 * k] - lo, x[8 * s + 2 * k + 1] - hi);
     }
     return rest;
 }

@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
     __shared__ float wave_weight[STREAM_WAVES][STREAM_ROWS];
     const u32 lane = threadIdx.x % 64;
     const u32 half = lane / 32;
-    const u32 wave = static_cast<u32>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)));
+    const u32 wave = uniform(threadIdx.x / 64);
     char* const keys = lds + wave * 2 * TILE_BYTES;
     char* const values = keys + TILE_BYTES;
     const u32 id = die_order(blockIdx.x, gridDim.x);
@@ -76,10 +76,10 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
     }
     for (; tile < end; tile += STREAM_WAVES)
     {
-        w.template put<T>(keys, next_keys);
-        w.template put<V>(values, next_values);
-        const typename wave_type::place current = now;
         const u32 taking = in;
+        const typename wave_type::scales scales = w.ready(now, ((taking >> (lane % 32)) & 1) != 0);
+        w.template put<true>(keys, next_keys, 1.0F);
+        w.template put<false>(values, next_values, scales.value_scale);
         now = next;
         next.block = after.block;
         in = w.taking_part(now, tile + STREAM_WAVES);
@@ -100,16 +100,6 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
         {
             score = mfma<T>::run(tile_row<DP>(keys, lane % 32, s), query[s], score);
         }
-        if constexpr (CACHE)
-        {
-            const float lo = w.of_sixteen(current.key_scale, 0);
-            const float hi = w.of_sixteen(current.key_scale, 1);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                score[i] *= i < 8 ? lo : hi;
-            }
-        }
         if (taking != ~0U)
         {
             const u32 bits = taking >> (4 * half);
@@ -119,18 +109,25 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
                 score[i] = ((bits >> (8 * (i / 4) + i % 4)) & 1) != 0 ? score[i] : -__builtin_inff();
             }
         }
-        float most = score[0];
+        // the factors of the two sixteens of the tile: registers 0 .. 7 and 8 .. 15
+        const float factor[2] = {CACHE ? w.of_sixteen(scales.key_factor, 0) : a.exponent_scale,
+                                 CACHE ? w.of_sixteen(scales.key_factor, 1) : a.exponent_scale};
+        float largest[2] = {score[0], score[8]};
 #pragma unroll
-        for (int i = 1; i < 16; ++i)
+        for (int i = 1; i < 8; ++i)
         {
-            most = fmaxf(most, score[i]);
+            largest[0] = fmaxf(largest[0], score[i]);
+            largest[1] = fmaxf(largest[1], score[8 + i]);
         }
-        most = fmaxf(most, other_half(most)) * a.exponent_scale;
-        most = fmaxf(most, top);
-        const float base = most == -__builtin_inff() ? 0.0F : most;
-        if (__any(most > top))
+        float most = fmaxf(largest[0] * factor[0], largest[1] * factor[1]);
+        most = fmaxf(most, other_half(most));
+        // The reference of the exponents follows the maximum only where that has grown by more than 8:
+        // weights stay below 2^8, and the sums are seldom rescaled.
+        if (__any(most > top + 8.0F))
         {
-            const float shrink = __builtin_amdgcn_exp2f(top - base);
+            asm volatile(""); // stays a branch
+            most = fmaxf(most, top);
+            const float shrink = __builtin_amdgcn_exp2f(top - (most == -__builtin_inff() ? 0.0F : most));
             weight *= shrink;
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
@@ -139,24 +136,19 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
             }
             top = most;
         }
-        float part = 0.0F;
+        const float base = top == -__builtin_inff() ? 0.0F : top;
+        float part[2] = {0.0F, 0.0F};
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int g = 0; g < 2; ++g)
         {
-            score[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], a.exponent_scale, -base));
-            part += score[i];
-        }
-        weight += part;
-        if constexpr (CACHE)
-        {
-            // a sixteen without a state that takes part: its weights are zero, its scale may be anything
-            const float lo = (taking & 0xFFFFU) != 0 ? w.of_sixteen(current.value_scale, 0) : 0.0F;
-            const float hi = (taking >> 16) != 0 ? w.of_sixteen(current.value_scale, 1) : 0.0F;
+            const float from = CACHE ? w.of_sixteen(scales.mantissa_log, g) - base : -base;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 8 * g; i < 8 * g + 8; ++i)
             {
-                score[i] *= i < 8 ? lo : hi;
+                score[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], factor[g], from));
+                part[g] += score[i];
             }
+            weight = CACHE ? __builtin_fmaf(part[g], w.of_sixteen(scales.mantissa_inverse, g), weight) : weight + part[g];
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -165,7 +157,7 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
             vuint4 rest;
             if constexpr (wave_type::PIECES)
             {
-                rest = operand_rest(score, s, p);
+                rest = operand_rest<V>(score, s, p);
             }
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)

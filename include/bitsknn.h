@@ -439,9 +439,10 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
  * required.  Every sum has one order: the same call gives the same bits.
  *   workspace      bitsknn_cross_attention_backward_workspace_bytes bytes, 16-byte aligned; a smaller
  *                  one is BITSKNN_ERR_INVALID where it does not hold a float per row
- * Weights and their derivatives are rounded to the vectors' type for the products, sums are fp32 and
- * the results are rounded once.  Fp16: derivatives of the scores below 2^-24 vanish, so gradients want
- * a loss scale that keeps them above it.
+ * Weights and derivatives of the scores are rounded to the vectors' type for the products (for the
+ * queries' gradient the derivatives enter in two pieces), sums are fp32 and the results are rounded once.
+ * Fp16: derivatives of the scores below 2^-24 vanish, so gradients want a loss scale that keeps them
+ * above it.  No gradient may share memory with an input.
  */
 size_t bitsknn_cross_attention_backward_workspace_bytes(const bitsknn_attention_shape* shape);
 int bitsknn_cross_attention_backward(const bitsknn_attention_shape* shape, const bitsknn_rows* grad_out,
