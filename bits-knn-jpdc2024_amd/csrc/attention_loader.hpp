@@ -265,16 +265,17 @@ __device__ __forceinline__ vuint4 operand_rest(const vfloat16& x, int s, vuint4 
 #pragma unroll
     for (int k = 0; k < 4; ++k)
     {
+        const u32 word = p[k]; // a copy: a bit cast of an element in place reads the vector's first
         float lo;
         float hi;
         if constexpr (std::is_same_v<V, __bf16>)
         {
-            lo = __builtin_bit_cast(float, p[k] << 16);
-            hi = __builtin_bit_cast(float, p[k] & 0xFFFF0000U);
+            lo = __builtin_bit_cast(float, word << 16);
+            hi = __builtin_bit_cast(float, word & 0xFFFF0000U);
         }
         else
         {
-            const auto both = __builtin_bit_cast(typename mfma<V>::v2, p[k]);
+            const auto both = __builtin_bit_cast(typename mfma<V>::v2, word);
             lo = static_cast<float>(both[0]);
             hi = static_cast<float>(both[1]);
         }
