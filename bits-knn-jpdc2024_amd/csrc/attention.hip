@@ -13,11 +13,8 @@ namespace
 
 constexpr u32 WAVE_ROWS = 32; // rows per wave: the columns of a matrix product
 
-#ifndef TW
-#define TW 8
-#endif
 // Waves that share a tile.  In 256 dimensions a wave needs all the registers of its quarter of the unit.
-constexpr u32 tile_waves(int padded_dim) { return padded_dim <= 128 ? TW : 4; }
+constexpr u32 tile_waves(int padded_dim) { return padded_dim <= 128 ? 8 : 4; }
 // States per tile: five tiles have to fit LDS.
 constexpr u32 tile_keys(int padded_dim) { return padded_dim <= 128 ? 64 : 32; }
 constexpr u32 tile_rows(int padded_dim) { return WAVE_ROWS * tile_waves(padded_dim); }
@@ -97,6 +94,16 @@ __device__ __forceinline__ void store_out(const attention_args& a, const row_sta
     }
 }
 
+// Sequences of one length: neighbours, which read the same states, on one die.  Of different lengths: the
+// tiles of each dealt out to all dies, so that they end together (101 against 109 us for 4 x 16/4 heads,
+// 512 rows over up to 4096 states of the cache; with one length 568 against 551 us for 4 x 16/4 heads, 2048 x
+// 8192).
+template <bool CACHE>
+__device__ __forceinline__ u32 tile_order(const attention_args& a)
+{
+    return CACHE || a.counts != nullptr ? blockIdx.x : die_order(blockIdx.x, gridDim.x);
+}
+
 // Bound by the matrix instructions.  A workgroup's waves hold 32 rows each and share tiles of states in
 // LDS.  A wave goes through the states by 32: one step takes the scores of the next 32 on the matrix
 // path, turns those of the present 32 into weights on the vector unit meanwhile, multiplies them with
@@ -105,7 +112,7 @@ __device__ __forceinline__ void store_out(const attention_args& a, const row_sta
 // the slowest wave may still read the last values of the tile before) ahead of a tile's last step, which
 // already reads the next keys: one barrier per tile.
 template <typename T, int DP, bool CACHE>
-__global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attention_tile_kernel(const attention_args a)
+__global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 64 ? 4 : (DP <= 128 ? 2 : 1)) attention_tile_kernel(const attention_args a)
 {
     constexpr u32 THREADS = 64 * tile_waves(DP);
     constexpr u32 KEYS = tile_keys(DP);
@@ -121,11 +128,11 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
         float mantissa_log[KEYS / 16];
         float mantissa_inverse[KEYS / 16];
     };
-    __shared__ __attribute__((aligned(16))) char lds[5 * TILE_BYTES];
+    __shared__ __attribute__((aligned(512))) char lds[5 * TILE_BYTES];
     __shared__ __attribute__((aligned(16))) tile_info infos[3];
     const u32 lane = threadIdx.x & 63;
     const u32 half = lane / 32;
-    const u32 id = die_order(blockIdx.x, gridDim.x);
+    const u32 id = tile_order<CACHE>(a);
     const u32 row_tile = id % a.row_tiles;
     const u32 split = id / a.row_tiles % a.splits;
     const u32 head = id / a.row_tiles / a.splits % static_cast<u32>(a.state_heads);
@@ -185,10 +192,14 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
         w.template load<true>(next_keys, now, t, in);
         w.template load<false>(next_values, now, t, in);
     };
+    // a lane's places in a tile, in one register each
+    const u32 row_at = row_address<DP>(lds, lane % 32);
+    const u32 first_at = column_address<DP>(lds, 0);
+    const u32 second_at = column_address<DP>(lds, 8);
     // scores of the 32 states u of a tile
     const auto scores_of = [&](u32 k, u32 v, u32 u) {
         const tile_info& t = infos[v];
-        const char* keys = lds + k * TILE_BYTES;
+        const u32 key_row = row_at + k * TILE_BYTES + u * 32 * DP * 2;
         vfloat16 score;
 #pragma unroll
         for (u32 g = 0; g < 4; ++g)
@@ -201,9 +212,9 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
             }
         }
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+        for (u32 s = 0; s < DP / 16; ++s)
         {
-            score = mfma<T>::run(tile_row<DP>(keys, 32 * u + lane % 32, s), query[s], score);
+            score = mfma<T>::run(lds_read<vuint4>(key_row ^ (32 * s)), query[s], score);
         }
         return score;
     };
@@ -267,7 +278,14 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
                 __syncthreads();
             }
             const tile_info& t = infos[value_place];
-            const char* values = lds + (2 + value_place) * TILE_BYTES;
+            const u32 first = first_at + (2 + value_place) * TILE_BYTES + u * 32 * DP * 2;
+            const u32 second = second_at + (2 + value_place) * TILE_BYTES + u * 32 * DP * 2;
+            if constexpr (!CACHE)
+            {
+                // the wave at the matrix path goes first (537 against 551 us for 4 x 16/4 heads, 2048 x
+                // 8192; the cache's, with more of its time on the vector unit: 115 against 109 us)
+                __builtin_amdgcn_s_setprio(1);
+            }
             const vfloat16 next_score = last ? scores_of(next_key_place, next_value_place, 0) : scores_of(key_place, value_place, u + 1);
 #pragma unroll
             for (u32 g = 0; g < 2; ++g)
@@ -284,24 +302,29 @@ __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 128 ? 2 : 1) attent
                 st.weight = CACHE ? __builtin_fmaf(weight, t.mantissa_inverse[2 * u + g], st.weight) : st.weight + weight;
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (u32 s = 0; s < 2; ++s)
             {
-                const vuint4 p = operand<V>(score, s);
+                const vuint4 p = operand<V>(score, static_cast<int>(s));
                 vuint4 rest;
                 if constexpr (loader::PIECES)
                 {
-                    rest = operand_rest<V>(score, s, p);
+                    rest = operand_rest<V>(score, static_cast<int>(s), p);
                 }
 #pragma unroll
-                for (int m = 0; m < DP / 32; ++m)
+                for (u32 m = 0; m < DP / 32; ++m)
                 {
-                    const vuint4 v = tile_column<DP>(values, 2 * u + s, m);
+                    const u32 rows_on = 16 * s * DP * 2;
+                    const vuint4 v = read_column((first ^ (64 * m)) + rows_on, (second ^ (64 * m)) + rows_on);
                     st.sum[m] = mfma<V>::run(v, p, st.sum[m]);
                     if constexpr (loader::PIECES)
                     {
                         st.sum[m] = mfma<V>::run(v, rest, st.sum[m]);
                     }
                 }
+            }
+            if constexpr (!CACHE)
+            {
+                __builtin_amdgcn_s_setprio(0);
             }
             follow(next_score, last ? next_value_place : value_place, last ? 0 : u + 1);
             score = next_score;
@@ -383,11 +406,15 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const attention_arg
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
 
-// Few rows stream past 32 at a time, more of them share tiles of 128 rows.
+// Up to two tiles of 32 rows stream the states past, more rows share tiles of states (48 rows, streamed:
+// 22 us; 80 rows in tiles: 23 us; 4 x 4 heads over 4096 states x 64).
 constexpr u32 MOST_STREAM_ROWS = 64;
 
-// two per compute unit (1024 and 2048: 3 and 6 us longer for 64 sequences of 32 heads over 8192 states)
-constexpr size_t WANTED_WORKGROUPS = 512;
+// Two workgroups per compute unit stream (1024 and 2048 in all: 3 and 6 us longer than 512 for 64
+// sequences of 32 heads over 8192 states); of those that share tiles one fills a unit (512 in all: 122
+// against 109 us for 4 x 16/4 heads, 512 rows over 4096 states of the cache).
+constexpr size_t WANTED_STREAMS = 512;
+constexpr size_t WANTED_TILES = 256;
 
 bool streams(size_t rows) { return rows <= MOST_STREAM_ROWS; }
 
@@ -398,17 +425,19 @@ u32 row_tiles_of(size_t rows, int dim)
 }
 
 // How many ranges the states are cut into: as many as give the GPU enough workgroups, at least 512
-// states each (a join of ranges costs a launch: 12.1 us for three of 333 states, 12.6 us for one of 1000).
+// states each where they stream (a join of ranges costs a launch: 12.1 us for three of 333 states, 12.6 us
+// for one of 1000), 256 where rows share tiles (128: 39 against 31 us for 3 x 12/4 heads, 333 x 1001).
 u32 wanted_splits(const bitsknn_attention_shape& s)
 {
     const size_t rows = static_cast<size_t>(s.queries) * static_cast<u32>(s.query_heads / s.state_heads);
     const size_t groups = static_cast<size_t>(s.batch) * static_cast<u32>(s.state_heads) * row_tiles_of(rows, s.dim);
-    const size_t most = static_cast<size_t>(s.states) / 512;
-    if (groups == 0 || groups >= WANTED_WORKGROUPS)
+    const size_t wanted = streams(rows) ? WANTED_STREAMS : WANTED_TILES;
+    const size_t most = static_cast<size_t>(s.states) / (streams(rows) ? 512 : 256);
+    if (groups == 0 || groups >= wanted)
     {
         return 1;
     }
-    size_t splits = (WANTED_WORKGROUPS + groups - 1) / groups;
+    size_t splits = (wanted + groups - 1) / groups;
     splits = splits < most ? splits : most;
     splits = splits < 64 ? splits : 64;
     return splits < 1 ? 1 : static_cast<u32>(splits);
