@@ -32,7 +32,8 @@ inline int check_shape(const char* name, const bitsknn_attention_shape& s)
         return fail(BITSKNN_ERR_INVALID, "%s: %d query heads do not share %d state heads", name, s.query_heads,
                     s.state_heads);
     }
-    if (!(s.scale > 0.0F) || !(s.scale <= 3.402823466e38F))
+    // the kernels use it times log2(e)
+    if (!(s.scale > 0.0F) || !(s.scale * LOG2E <= 3.402823466e38F))
     {
         return fail(BITSKNN_ERR_INVALID, "%s: scale %g is not positive and finite", name, static_cast<double>(s.scale));
     }

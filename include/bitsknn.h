@@ -387,13 +387,13 @@ int bitsknn_fused_status(void* stream);
  *   dim            1 <= dim <= 256, a multiple of 8; vectors start on 16-byte boundaries
  *   queries        rows per query head, may be 0
  *   states         states per state head, may be 0
- *   scale          positive and finite
+ *   scale          positive, and finite when multiplied by log2(e)
  *   counts         NULL, or batch int32: sequence b has the states [0, counts[b]) (a count below 0 is
  *                  0, one above `states` is `states`)
  *   mask           NULL, or batch rows of `states` bytes, row stride mask_stride: a state whose byte is
  *                  zero takes no part
  * Keys and values that take no part are not used, whatever they hold (NaN and infinities too).
- *   out            as queries, no two vectors overlapping
+ *   out            as queries, no two vectors overlapping, sharing no memory with an input
  *   lse            NULL, or batch x query_heads x queries floats, contiguous
  *   workspace      16-byte aligned device memory for partial sums.  Where the rows are too few to fill
  *                  the GPU the states are cut into ranges that separate workgroups read;
@@ -504,8 +504,10 @@ int bitsknn_cache_store(const bitsknn_state_cache* cache, int32_t type, int32_t 
  * that ceil(states / block) entries of the table name; place j takes part if j < counts[b] (where counts
  * is given), its block is named, and its place in the block is below the block's block_counts.  A block
  * named twice counts twice.  shape->state_heads and shape->dim are the cache's; scales as stored or any
- * others.  The codes are multiplied as they stand and the scales are applied in fp32.  Arguments else,
- * workspace, results and errors as for bitsknn_cross_attention.
+ * others that are not negative.  Keys are multiplied as their codes stand and their scale is applied in
+ * fp32; values enter times the power of two of their scale, exactly (below 2^-126 they may count as zero),
+ * and the rest of the scale is applied to the weights.  Arguments else, workspace, results and errors as
+ * for bitsknn_cross_attention.
  */
 size_t bitsknn_cached_attention_workspace_bytes(const bitsknn_attention_shape* shape);
 int bitsknn_cached_attention(const bitsknn_attention_shape* shape, const bitsknn_rows* queries,

@@ -38,6 +38,7 @@ SHAPES = [
     (dict(scale=-1.0), "INVALID", "not positive and finite"),
     (dict(scale=float("inf")), "INVALID", "not positive and finite"),
     (dict(scale=float("nan")), "INVALID", "not positive and finite"),
+    (dict(scale=3e38), "INVALID", "not positive and finite"),
     (dict(queries=1 << 30, query_heads=8), "UNSUPPORTED", "too many rows"),
     (dict(states=0x7FFFFFFF), "UNSUPPORTED", "too many rows"),
 ]
