@@ -403,6 +403,7 @@ def _rows(t):
 
 def _attention_shape(queries, state_heads, states, scale):
     batch, heads, rows, dim = queries.shape
+    assert states < 2 ** 31 and max(queries.shape) < 2 ** 31  # ctypes would cut them silently
     return AttentionShape(_attention_type(queries.dtype), dim, batch, heads, state_heads, rows, states,
                           dim ** -0.5 if scale is None else scale)
 
