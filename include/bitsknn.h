@@ -377,8 +377,9 @@ int bitsknn_fused_status(void* stream);
  * search finds or an encoder leaves behind.  For query row i of head h, with s_j = scale * q_i . k_j
  * over the states j that take part,
  *     lse_i = log(sum_j exp(s_j)),   out_i = sum_j exp(s_j - lse_i) v_j
- * in one pass over the states; no score is written to memory.  A row without any state has out = 0
- * and lse = -inf.  No counterpart in the reference.
+ * in one pass over the states; no score is written to memory.  A row without any state, or whose
+ * scores are all minus infinity, has out = 0 and lse = -inf, whatever its query holds.  No counterpart in
+ * the reference.
  *
  * Vectors are 16-bit floats in batch x heads x rows x dim, every vector contiguous, the other strides
  * the caller's (bitsknn_rows, in elements; an input's stride may be 0).  query_heads is a multiple of

@@ -207,3 +207,48 @@ def test_replayed_from_a_graph(bk, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), replay
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [3, 64, 65, 200])
+@pytest.mark.parametrize("kind", ["counts", "mask"])
+def test_rows_without_states_whatever_the_queries_hold(bk, dev, dtype, dim, rows, kind):
+    """A padded batch: sequence 1 has no state, its queries hold NaN and infinities.  Also with enough
+    states for several ranges."""
+    for n in (70, 1100):
+        queries, keys, values = _inputs(dev, (3, 1, 1, rows, n, dim), dtype, 15)
+        queries[1, :, 0::3] = math.nan
+        queries[1, :, 1::3, 0] = math.inf
+        queries[1, :, 2::3, -1] = -math.inf
+        counts = torch.tensor([n, 0, n // 2 + 1], dtype=torch.int32, device=dev)
+        mask = torch.arange(n, device=dev)[None] < counts[:, None]
+        gone = ~mask[:, None, :, None]
+        keys, values = keys.masked_fill(gone, math.nan), values.masked_fill(gone, math.inf)
+        out, lse = bk.cross_attention(queries, keys, values, **({"counts": counts} if kind == "counts" else {"mask": mask}))
+        assert (out[1] == 0).all() and (lse[1] == -math.inf).all()
+        for b in (0, 2):
+            want = ref.attention(queries[b:b + 1], keys[b:b + 1], values[b:b + 1], dim ** -0.5, mask[b:b + 1].cpu())
+            ref.check(out[b:b + 1], want[0], want[2], "out")
+            ref.check(lse[b:b + 1], want[1], want[3], "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [64, 65])
+def test_scores_of_minus_infinity(bk, dev, dtype, rows):
+    """Rows all of whose scores are minus infinity count as rows without states, whatever is masked; one
+    finite score decides a row."""
+    queries, keys, values = _inputs(dev, (1, 1, 1, rows, 150, 64), dtype, 16)
+    keys[..., 0] = keys[..., 0].abs() + 1
+    keys[0, 0, 77, 0] = 0.0
+    queries[..., 0] = -math.inf
+    mask = torch.rand((1, 150), generator=torch.Generator().manual_seed(5)) < 0.7
+    mask[0, 77] = False
+    out, lse = bk.cross_attention(queries, keys, values, mask=mask.to(dev))
+    assert (out == 0).all() and (lse == -math.inf).all()
+    queries[..., 0] = 1.0
+    keys[..., 0] = -math.inf
+    mask[0, 77] = True
+    keys[0, 0, 77, 0] = 0.0
+    out, lse = bk.cross_attention(queries, keys, values, mask=mask.to(dev))
+    assert torch.equal(out, values[:, :, 77:78].expand_as(out)) and lse.isfinite().all()

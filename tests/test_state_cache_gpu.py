@@ -338,3 +338,22 @@ def test_search_store_and_read_together(bk, dev):
     _check(bk, dev, queries, cache, near.cpu())
     whole, _ = bk.cached_attention(queries.to(dev), cache, names.to(dev).expand(40, -1))
     assert not torch.equal(got, whole)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [3, 64, 65, 200])
+def test_sequences_without_states_whatever_the_queries_hold(bk, dev, dtype, dim, rows):
+    """No entry names a block, all blocks are empty, or the count is 0; the queries hold NaN and infinities."""
+    shape = (4, 1, 1, rows, 40, dim, 32)
+    cache, table = _cache(bk, dev, shape, 9)
+    queries = _queries(shape, dtype)
+    queries[1:, :, 0::3] = math.nan
+    queries[1:, :, 1::3, 0] = math.inf
+    queries[1:, :, 2::3, -1] = -math.inf
+    table[1] = torch.tensor([-1, 2 ** 31 - 1]).repeat(20)
+    cache.block_counts[table[2].long()] = 0
+    counts = torch.tensor([1280, 1280, 1280, 0], dtype=torch.int32)
+    out, lse = bk.cached_attention(queries.to(dev), cache, table.to(dev), counts.to(dev))
+    assert (out[1:] == 0).all() and (lse[1:] == -math.inf).all()
+    _check(bk, dev, queries[:1], cache, table[:1])
