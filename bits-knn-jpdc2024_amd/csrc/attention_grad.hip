@@ -446,6 +446,15 @@ __global__ void __launch_bounds__(ROW_THREADS, DP <= 128 ? 2 : 1) attention_grad
     }
     if (mine)
     {
+        if (top == __builtin_inff())
+        {
+            // a row without any state: its zero weights times what it holds may be anything
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+            {
+                sum[n] = vfloat16{};
+            }
+        }
         store_vector<T, DP>(g.grad_queries.data + 2 * row_offset(g.grad_queries, a, b, head, row), sum, a.scale,
                             static_cast<u32>(a.dim));
     }

@@ -434,8 +434,8 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
 /*
  * Gradients of bitsknn_cross_attention's out with respect to queries, keys and values, from what the
  * forward call read and returned and the gradient of out (that of lse is taken as zero).  States that
- * take no part get a gradient of zero; so do rows without any state.  Shared heads' gradients are summed
- * over the heads that share them; inputs that a stride of 0 repeats get one gradient per repetition
+ * take no part get a gradient of zero; so do rows without any state, whatever they and their incoming
+ * gradients hold.  Shared heads' gradients are summed over the heads that share them; inputs that a stride of 0 repeats get one gradient per repetition
  * (the gradients' vectors must not overlap).  counts, mask and scale as in the forward call, lse
  * required.  Every sum has one order: the same call gives the same bits.
  *   workspace      bitsknn_cross_attention_backward_workspace_bytes bytes, 16-byte aligned; a smaller

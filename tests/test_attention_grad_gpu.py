@@ -249,3 +249,33 @@ def test_step_replayed_from_a_graph(bk, dev):
         torch.cuda.synchronize()
         for x, y in zip([out, lse] + grads, [eager_out, eager_lse] + list(want)):
             assert torch.equal(x, y), replay
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [3, 64, 65, 200])
+@pytest.mark.parametrize("kind", ["counts", "mask"])
+def test_rows_without_states_whatever_they_hold(bk, dev, dtype, dim, rows, kind):
+    """Sequence 1 has no state; its queries and its incoming gradients hold NaN and infinities."""
+    n = 100
+    grad_out, queries, keys, values = _inputs(dev, (3, 1, 1, rows, n, dim), dtype, 60)
+    for x, shift in ((queries, 0), (grad_out, 1)):
+        x[1, :, shift::3] = math.nan
+        x[1, :, (shift + 1) % 3::3, 0] = math.inf
+        x[1, :, (shift + 2) % 3::5, -1] = -math.inf
+    counts = torch.tensor([n, 0, n // 2 + 1], dtype=torch.int32, device=dev)
+    mask = torch.arange(n, device=dev)[None] < counts[:, None]
+    part = {"counts": counts} if kind == "counts" else {"mask": mask}
+    out = torch.zeros_like(queries)
+    lse = torch.full(queries.shape[:3], -math.inf, device=dev)
+    for b in (0, 2):
+        one, one_lse = bk.cross_attention(queries[b:b + 1], keys[b:b + 1], values[b:b + 1], mask=mask[b:b + 1])
+        out[b], lse[b] = one[0], one_lse[0]
+    got = bk.cross_attention_backward(grad_out, queries, keys, values, out, lse, **part)
+    for x in got:
+        assert (x[1] == 0).all()
+    for b in (0, 2):
+        s = slice(b, b + 1)
+        wants = ref.gradients(grad_out[s], queries[s], keys[s], values[s], out[s], lse[s], dim ** -0.5, mask[s].cpu())
+        for name, one, (want, bound) in zip(("queries", "keys", "values"), got, wants):
+            ref.check(one[s], want, bound, name)
