@@ -76,6 +76,65 @@ __device__ __forceinline__ float exponent_base(float lse)
     return lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
 }
 
+// Derivatives enter the products in the vectors' type.  fp16 ends at 65504, which P (dP - delta) passes
+// where the gradient, smaller by the scale, need not.  One infinite derivative leaves no number in its row's
+// or state's sums, so a walk is taken as it comes and its sums are looked at; where a workgroup finds such a
+// sum, it walks again in range: a lane's derivatives, all of one row or all of one state, are multiplied by a
+// power of two (1 as long as they fit) that brings the largest so far below 2^15, exactly in fp32, and the
+// sums follow it.  What falls below fp16's least number then is below 2^-39 of the largest, and a row or
+// state whose derivatives fit gets the same bits in either walk.  (All walks in
+// range: 30.3 against 26.0 us for 2 x 8/2 heads, 65 x 257 x 64, 440 against 370 us for 2 x 16/4 heads, 2048 x
+// 4096 x 64; bf16 has the exponents of fp32 and needs none of this.)
+template <typename T>
+constexpr bool RANGE = std::is_same_v<T, _Float16>;
+
+// the sums times a power of two
+template <int DP>
+__device__ __forceinline__ void scale_sums(vfloat16 (&sum)[DP / 32], float power)
+{
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+    {
+        if constexpr (DP == 256)
+        {
+            // they stay in the accumulation registers before and after (194 registers spilled otherwise)
+            asm volatile("" : "+a"(sum[n]));
+        }
+        sum[n] *= power;
+        if constexpr (DP == 256)
+        {
+            asm volatile("" : "+a"(sum[n]));
+        }
+    }
+}
+
+// derivatives weight * slope: the power goes into the slopes
+template <int DP>
+__device__ __forceinline__ void keep_in_range(const vfloat16& weight, vfloat16& slope, float& power, vfloat16 (&sum)[DP / 32])
+{
+    float most = 0.0F;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+    {
+        most = fmaxf(most, __builtin_fabsf(weight[i] * slope[i]));
+    }
+    most = fmaxf(most, other_half(most));
+    if (most * power > 65504.0F)
+    {
+        // most is in [2^e, 2^(e + 1)), e >= 15: times 2^(14 - e)
+        const u32 exponent = __builtin_bit_cast(u32, most) >> 23;
+        const float next = __builtin_bit_cast(float, (2 * 127 + 14 - exponent) << 23);
+        scale_sums<DP>(sum, next / power);
+        power = next;
+    }
+    slope *= power;
+}
+
+__device__ __forceinline__ bool finite(float x)
+{
+    return (__builtin_bit_cast(u32, x) & 0x7F800000U) != 0x7F800000U;
+}
+
 // Steps of 32 rows of queries and incoming gradients into LDS, and what a row's scores need: the base of
 // its exponents and its delta.  Rows behind the last one are zero with weights of zero.
 template <int DP>
@@ -225,15 +284,19 @@ __global__ void __launch_bounds__(64 * state_waves(DP), DP <= 128 ? 2 : 1) atten
     }
     vfloat16 key_sum[DP / 32];
     vfloat16 value_sum[DP / 32];
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-    {
-        key_sum[n] = vfloat16{};
-        value_sum[n] = vfloat16{};
-    }
     const u32 steps = __syncthreads_or(in) != 0 ? (a.rows + STEP_ROWS - 1) / STEP_ROWS : 0;
-    if (steps > 0)
-    {
+    const auto walk = [&](auto in_range) {
+        float power = 1.0F; // of the lane's state: times key_sum
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+        {
+            key_sum[n] = vfloat16{};
+            value_sum[n] = vfloat16{};
+        }
+        if (steps == 0)
+        {
+            return;
+        }
         row_loader<DP> rows{g, b, head};
         rows.fetch();
         rows.put(lds, lds + TILE_BYTES, bases[0], deltas[0]);
@@ -274,11 +337,15 @@ __global__ void __launch_bounds__(64 * state_waves(DP), DP <= 128 ? 2 : 1) atten
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                 {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i + j], a.exponent_scale, -top[j]));
-                    p[i + j] = x;
-                    slope[i + j] = x * (slope[i + j] - d[j]);
+                    p[i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i + j], a.exponent_scale, -top[j]));
+                    slope[i + j] -= d[j];
                 }
             }
+            if constexpr (in_range())
+            {
+                keep_in_range<DP>(p, slope, power, key_sum);
+            }
+            slope *= p;
             const vuint4 weight[2] = {operand<T>(p, 0), operand<T>(p, 1)};
             const vuint4 change[2] = {operand<T>(slope, 0), operand<T>(slope, 1)};
 #pragma unroll
@@ -296,6 +363,18 @@ __global__ void __launch_bounds__(64 * state_waves(DP), DP <= 128 ? 2 : 1) atten
             char* const other = lds + (1 - place) * 2 * TILE_BYTES;
             rows.put(other, other + TILE_BYTES, bases[1 - place], deltas[1 - place]);
             __syncthreads();
+        }
+        if constexpr (in_range())
+        {
+            scale_sums<DP>(key_sum, 1.0F / power);
+        }
+    };
+    walk(std::false_type{});
+    if constexpr (RANGE<T>)
+    {
+        if (__syncthreads_or(in && !finite(key_sum[0][0])) != 0)
+        {
+            walk(std::true_type{});
         }
     }
     if (state >= a.states)
@@ -350,11 +429,6 @@ __global__ void __launch_bounds__(ROW_THREADS, DP <= 128 ? 2 : 1) attention_grad
     const float top = mine ? exponent_base(a.lse[flat]) : __builtin_inff();
     const float delta = mine ? g.delta[flat] : 0.0F;
     vfloat16 sum[DP / 32];
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-    {
-        sum[n] = vfloat16{};
-    }
     const u32 count = uniform(state_count(a, b));
     const u32 tiles = (count + KEYS - 1) / KEYS;
     const loader w{a, b, head, count};
@@ -376,73 +450,99 @@ __global__ void __launch_bounds__(ROW_THREADS, DP <= 128 ? 2 : 1) attention_grad
             starts[place][threadIdx.x] = ((in >> threadIdx.x) & 1) != 0 ? 0.0F : -__builtin_inff();
         }
     };
-    if (tiles > 0)
-    {
-        w.look_up_state(next, 0);
-        fetch(0);
-        put(0);
-        __syncthreads();
-    }
     const u32 row_at = row_address<DP>(lds, lane % 32);
     const u32 first_at = column_address<DP>(lds, 0);
     const u32 second_at = column_address<DP>(lds, 8);
-    for (u32 tile = 0; tile < tiles; ++tile)
-    {
-        const u32 place = tile % 2;
-        fetch(tile + 1);
-#pragma unroll 1
-        for (u32 u = 0; u < KEYS / 32; ++u)
+    const auto walk = [&](auto in_range) {
+        float power = 1.0F; // of the lane's row: times sum
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
         {
-            const u32 at = place * 2 * TILE_BYTES + u * 32 * DP * 2;
-            u32 row_to = row_at + at;
-            u32 first = first_at + at;
-            u32 second = second_at + at;
-            // hidden from the compiler, as in the walk by states
-            asm volatile("" : "+v"(row_to), "+v"(first), "+v"(second));
-            vfloat16 p;
-            vfloat16 slope = {};
-#pragma unroll
-            for (u32 q = 0; q < 4; ++q)
-            {
-                const vfloat4 start = *reinterpret_cast<const vfloat4*>(starts[place] + 32 * u + 8 * q + 4 * half);
-#pragma unroll
-                for (u32 i = 0; i < 4; ++i)
-                {
-                    p[4 * q + i] = start[i];
-                }
-            }
-#pragma unroll
-            for (u32 s = 0; s < DP / 16; ++s)
-            {
-                p = mfma<T>::run(lds_read<vuint4>(row_to ^ (32 * s)), query[s], p);
-            }
-#pragma unroll
-            for (u32 s = 0; s < DP / 16; ++s)
-            {
-                slope = mfma<T>::run(lds_read<vuint4>((row_to ^ (32 * s)) + TILE_BYTES), grad[s], slope);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.exponent_scale, -top)) * (slope[i] - delta);
-            }
-            const vuint4 change[2] = {operand<T>(p, 0), operand<T>(p, 1)};
-            const vuint4 rest[2] = {operand_rest<T>(p, 0, change[0]), operand_rest<T>(p, 1, change[1])};
-#pragma unroll
-            for (u32 n = 0; n < DP / 32; ++n)
-            {
-#pragma unroll
-                for (u32 s = 0; s < 2; ++s)
-                {
-                    const u32 rows_on = 16 * s * DP * 2;
-                    const vuint4 k = read_column((first ^ (64 * n)) + rows_on, (second ^ (64 * n)) + rows_on);
-                    sum[n] = mfma<T>::run(k, change[s], sum[n]);
-                    sum[n] = mfma<T>::run(k, rest[s], sum[n]);
-                }
-            }
+            sum[n] = vfloat16{};
         }
-        put(1 - place);
-        __syncthreads();
+        if (tiles > 0)
+        {
+            w.look_up_state(next, 0);
+            fetch(0);
+            put(0);
+            __syncthreads();
+        }
+        for (u32 tile = 0; tile < tiles; ++tile)
+        {
+            const u32 place = tile % 2;
+            fetch(tile + 1);
+#pragma unroll 1
+            for (u32 u = 0; u < KEYS / 32; ++u)
+            {
+                const u32 at = place * 2 * TILE_BYTES + u * 32 * DP * 2;
+                u32 row_to = row_at + at;
+                u32 first = first_at + at;
+                u32 second = second_at + at;
+                // hidden from the compiler, as in the walk by states
+                asm volatile("" : "+v"(row_to), "+v"(first), "+v"(second));
+                vfloat16 p;
+                vfloat16 slope = {};
+#pragma unroll
+                for (u32 q = 0; q < 4; ++q)
+                {
+                    const vfloat4 start = *reinterpret_cast<const vfloat4*>(starts[place] + 32 * u + 8 * q + 4 * half);
+#pragma unroll
+                    for (u32 i = 0; i < 4; ++i)
+                    {
+                        p[4 * q + i] = start[i];
+                    }
+                }
+#pragma unroll
+                for (u32 s = 0; s < DP / 16; ++s)
+                {
+                    p = mfma<T>::run(lds_read<vuint4>(row_to ^ (32 * s)), query[s], p);
+                }
+#pragma unroll
+                for (u32 s = 0; s < DP / 16; ++s)
+                {
+                    slope = mfma<T>::run(lds_read<vuint4>((row_to ^ (32 * s)) + TILE_BYTES), grad[s], slope);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.exponent_scale, -top));
+                    slope[i] -= delta;
+                }
+                if constexpr (in_range())
+                {
+                    keep_in_range<DP>(p, slope, power, sum);
+                }
+                p *= slope;
+                const vuint4 change[2] = {operand<T>(p, 0), operand<T>(p, 1)};
+                const vuint4 rest[2] = {operand_rest<T>(p, 0, change[0]), operand_rest<T>(p, 1, change[1])};
+#pragma unroll
+                for (u32 n = 0; n < DP / 32; ++n)
+                {
+#pragma unroll
+                    for (u32 s = 0; s < 2; ++s)
+                    {
+                        const u32 rows_on = 16 * s * DP * 2;
+                        const vuint4 k = read_column((first ^ (64 * n)) + rows_on, (second ^ (64 * n)) + rows_on);
+                        sum[n] = mfma<T>::run(k, change[s], sum[n]);
+                        sum[n] = mfma<T>::run(k, rest[s], sum[n]);
+                    }
+                }
+            }
+            put(1 - place);
+            __syncthreads();
+        }
+        if constexpr (in_range())
+        {
+            scale_sums<DP>(sum, 1.0F / power);
+        }
+    };
+    walk(std::false_type{});
+    if constexpr (RANGE<T>)
+    {
+        if (__syncthreads_or(mine && top != __builtin_inff() && !finite(sum[0][0])) != 0)
+        {
+            walk(std::true_type{});
+        }
     }
     if (mine)
     {

@@ -443,7 +443,9 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
  * Weights and derivatives of the scores are rounded to the vectors' type for the products (for the
  * queries' gradient the derivatives enter in two pieces), sums are fp32 and the results are rounded once.
  * Fp16: derivatives of the scores below 2^-24 vanish, so gradients want a loss scale that keeps them
- * above it.  No gradient may share memory with an input.
+ * above it.  There is no such limit above: derivatives beyond 65504 are held times a power of two, and a
+ * gradient is infinite only where it is itself beyond fp16 (workgroups that meet such derivatives walk their
+ * part twice).  No gradient may share memory with an input.
  */
 size_t bitsknn_cross_attention_backward_workspace_bytes(const bitsknn_attention_shape* shape);
 int bitsknn_cross_attention_backward(const bitsknn_attention_shape* shape, const bitsknn_rows* grad_out,

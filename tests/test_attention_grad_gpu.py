@@ -279,3 +279,71 @@ def test_rows_without_states_whatever_they_hold(bk, dev, dtype, dim, rows, kind)
         wants = ref.gradients(grad_out[s], queries[s], keys[s], values[s], out[s], lse[s], dim ** -0.5, mask[s].cpu())
         for name, one, (want, bound) in zip(("queries", "keys", "values"), got, wants):
             ref.check(one[s], want, bound, name)
+
+
+def _check_large(bk, grad_out, queries, keys, values, scale, mask=None):
+    """fp16 gradients where derivatives of the scores are beyond fp16's largest number.  A derivative then
+    enters the products times a power of two of its row (queries) or state (keys) that brings the largest
+    to at least 2^14, so what vanishes below fp16's least number, 2^-25, is at most 2^-25 times
+    (largest / 2^14): added to the bound, for all rows and states."""
+    out, lse = bk.cross_attention(queries, keys, values, mask=mask, scale=scale)
+    keep = ref.taking_part(keys.shape[0], keys.shape[2], None, mask)
+    got = bk.cross_attention_backward(grad_out, queries, keys, values, out, lse, mask=mask, scale=scale)
+    torch.cuda.synchronize()
+    wants = ref.gradients(grad_out, queries, keys, values, out, lse, scale, keep)
+    b, hs, n, dim = keys.shape
+    share = queries.shape[1] // hs
+    q, g, o, l = (x.cpu().double() for x in (queries, grad_out, out, lse))
+    gone = ~keep[:, None, :, None]
+    k, v = (x.cpu().double().masked_fill(gone, 0.0).repeat_interleave(share, 1) for x in (keys, values))
+    weights = torch.exp(q @ k.mT * scale - l[..., None]).masked_fill(~keep[:, None, None, :], 0.0)
+    slope = (weights * (g @ v.mT - (g * o).sum(-1, keepdim=True))).abs()
+    by_row = slope.amax(-1, keepdim=True)
+    by_state = slope.amax(2).view(b, hs, share, n).amax(2).repeat_interleave(share, 1)[:, :, None]
+    assert float(by_row.max()) > 65504 and float(by_state.max()) > 65504  # what this is about
+    lost = [1.1 * 2.0 ** -25 * x / 2.0 ** 14 for x in (by_row, by_state)]
+    extra = [scale * lost[0] * k.abs().sum(2, keepdim=True),
+             scale * (lost[1].mT * q.abs().sum(2, keepdim=True)).view(b, hs, share, n, dim).sum(2), 0.0]
+    finite = [float((want.abs() < 60000).double().mean()) for want, _ in wants]
+    assert min(finite) > 0.5, finite
+    for name, one, (want, bound), more in zip(("queries", "keys", "values"), got, wants, extra):
+        ref.check(one, want, bound + more, name)
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 150, 128), (1, 2, 1, 40, 140, 256), (2, 2, 1, 90, 300, 64), (1, 8, 1, 33, 40, 72)])
+@pytest.mark.parametrize("power", [12, 13])
+def test_large_derivatives_in_fp16(bk, dev, shape, power):
+    grad_out, queries, keys, values = _inputs(dev, shape, torch.float16, 70)
+    _check_large(bk, grad_out * 2.0 ** power, queries, keys, values * 8, shape[-1] ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_derivatives_that_grow_in_fp16(bk, dev, dim):
+    """They leave fp16's range late in both walks, for some rows and states only; peaked weights."""
+    b, h, hs, q, n, d = shape = (2, 2, 1, 150, 260, dim)
+    grad_out, queries, keys, values = _inputs(dev, shape, torch.float16, 80)
+    grad_out = grad_out * torch.exp2(torch.linspace(-4, 12, q, device=dev))[:, None].half()
+    values = values * torch.exp2(torch.linspace(-4, 5, n, device=dev))[:, None].half()
+    grad_out[:, :, 5::7] = grad_out[:, :, 5::7] * 2.0 ** -14
+    mask = torch.rand((b, n), generator=torch.Generator().manual_seed(1)) < 0.8
+    _check_large(bk, grad_out, queries, keys, values, 2.0 * d ** -0.5, mask.to(dev))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_that_hold_no_numbers_spoil_their_own_gradients_only(bk, dev, dtype, dim):
+    """A NaN in a row's incoming gradient: NaN in its query's gradient and in those of the states that it
+    reads; the rows beside it and the other sequence as without it, large ones too."""
+    grad_out, queries, keys, values = _inputs(dev, (2, 2, 1, 70, 90, dim), dtype, 90)
+    grad_out = grad_out * 2.0 ** 11
+    grad_out[1, :, 5::9] = 0.0
+    out, lse = bk.cross_attention(queries, keys, values)
+    want = bk.cross_attention_backward(grad_out, queries, keys, values, out, lse)
+    grad_out[1, :, 5::9] = math.nan
+    got = bk.cross_attention_backward(grad_out, queries, keys, values, out, lse)
+    spoilt = torch.zeros(70, dtype=torch.bool, device=dev)
+    spoilt[5::9] = True
+    for x, y in zip(got, want):
+        assert torch.equal(x[0], y[0])
+    assert torch.equal(got[0][1, :, ~spoilt], want[0][1, :, ~spoilt])
+    assert got[0][1, :, spoilt].isnan().all() and got[1][1].isnan().all() and got[2][1].isnan().all()
