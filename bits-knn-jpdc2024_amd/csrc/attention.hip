@@ -474,18 +474,19 @@ template <typename T, int DP, bool CACHE>
 int launch(attention_args& a, size_t rows, u32 batch, hipStream_t stream)
 {
     const u64 blocks = static_cast<u64>(batch) * static_cast<u32>(a.state_heads) * a.splits * a.row_tiles;
-    if (blocks > MOST_WORKGROUPS || (rows + 3) / 4 > MOST_WORKGROUPS)
+    const u32 threads = 64 * (streams(a.rows) ? STREAM_WAVES : tile_waves(DP));
+    if (!fits_grid(blocks, threads) || (a.splits > 1 && !fits_grid((rows + 3) / 4, 256)))
     {
         return fail(BITSKNN_ERR_UNSUPPORTED, "attention: too many rows (%zu)", rows);
     }
     if (streams(a.rows))
     {
-        hipLaunchKernelGGL((attention_stream_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)),
-                           dim3(64 * STREAM_WAVES), 0, stream, a);
+        hipLaunchKernelGGL((attention_stream_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)), dim3(threads), 0,
+                           stream, a);
     }
     else
     {
-        hipLaunchKernelGGL((attention_tile_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)), dim3(64 * tile_waves(DP)), 0,
+        hipLaunchKernelGGL((attention_tile_kernel<T, DP, CACHE>), dim3(static_cast<u32>(blocks)), dim3(threads), 0,
                            stream, a);
     }
     BITSKNN_HIP_CHECK(hipGetLastError());

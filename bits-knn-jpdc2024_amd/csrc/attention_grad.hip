@@ -564,11 +564,18 @@ template <typename T, int DP>
 int launch(const attention_grad_args& g, size_t rows, u32 batch, hipStream_t stream)
 {
     const u64 groups = static_cast<u64>(batch) * static_cast<u32>(g.f.state_heads);
+    constexpr size_t per_group = 256 / (DP / 8);
+    const size_t delta_groups = (rows + per_group - 1) / per_group;
+    // all three before the first
+    if (!fits_grid(delta_groups, 256) || !fits_grid(groups * g.f.row_tiles, ROW_THREADS) ||
+        !fits_grid(groups * g.key_tiles, 64 * state_waves(DP)))
+    {
+        return fail(BITSKNN_ERR_UNSUPPORTED, "bitsknn_cross_attention_backward: too many rows");
+    }
     if (rows > 0)
     {
-        constexpr size_t per_group = 256 / (DP / 8);
-        hipLaunchKernelGGL((attention_delta_kernel<T, DP>), dim3(static_cast<u32>((rows + per_group - 1) / per_group)),
-                           dim3(256), 0, stream, g, rows);
+        hipLaunchKernelGGL((attention_delta_kernel<T, DP>), dim3(static_cast<u32>(delta_groups)), dim3(256), 0, stream, g,
+                           rows);
         BITSKNN_HIP_CHECK(hipGetLastError());
         hipLaunchKernelGGL((attention_grad_rows_kernel<T, DP>), dim3(static_cast<u32>(groups * g.f.row_tiles)),
                            dim3(ROW_THREADS), 0, stream, g);
@@ -655,12 +662,6 @@ extern "C" int bitsknn_cross_attention_backward(const bitsknn_attention_shape* s
     const int padded = s.dim <= 64 ? 64 : (s.dim <= 128 ? 128 : 256);
     a.row_tiles = (a.rows + GRAD_ROWS - 1) / GRAD_ROWS;
     g.key_tiles = (a.states + states_per_group(padded) - 1) / states_per_group(padded);
-    const u64 groups = static_cast<u64>(s.batch) * static_cast<u32>(hs);
-    if (groups * a.row_tiles > MOST_WORKGROUPS || groups * g.key_tiles > MOST_WORKGROUPS ||
-        (rows + 3) / 4 > MOST_WORKGROUPS)
-    {
-        return fail(BITSKNN_ERR_UNSUPPORTED, "%s: too many rows", name);
-    }
     a.counts = counts;
     a.mask = mask;
     a.mask_stride = static_cast<std::int64_t>(mask_stride);

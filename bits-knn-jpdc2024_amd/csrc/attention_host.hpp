@@ -9,8 +9,8 @@ namespace bitsknn
 namespace
 {
 
-// a grid holds fewer than 2^32 threads; 256 threads per workgroup
-constexpr u64 MOST_WORKGROUPS = (1U << 24) - 1;
+// Whether a launch can hold so many workgroups of so many threads: a grid has fewer than 2^32 threads.
+inline bool fits_grid(u64 groups, u64 threads) { return groups <= 0xFFFFFFFFULL / threads; }
 
 inline int check_shape(const char* name, const bitsknn_attention_shape& s)
 {

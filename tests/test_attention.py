@@ -181,3 +181,50 @@ def test_cached_attention_refusals(bk):
     status, text = _read(bk, out=_rows(bk, row_stride=0))
     assert status == bk.ERR_INVALID and "out: vectors overlap" in text
     assert _read(bk, shape=_shape(bk, queries=0), queries=bk.Rows(), out=bk.Rows())[0] == bk.OK
+
+
+# ---- launches that a grid cannot hold -----------------------------------------------------------------
+
+
+def _backward(bk, shape, lse=64, workspace=64, workspace_bytes=1 << 60):
+    L = bk.lib()
+    one = _rows(bk, batch_stride=1 << 20, head_stride=1 << 16, row_stride=256)
+    status = L.bitsknn_cross_attention_backward(shape, one, one, one, one, one, ctypes.c_void_p(lse), None, None, 0, one,
+                                                one, one, ctypes.c_void_p(workspace), workspace_bytes, None)
+    return status, L.bitsknn_last_error().decode()
+
+
+# A grid has fewer than 2^32 threads.  Workgroups of the walk by states: 512 threads from 72 to 128
+# dimensions, 256 else; of the walk by rows 256; of the rows' deltas 8, 16 or 32 threads per row.
+@pytest.mark.parametrize("change", [
+    dict(dim=128, batch=1 << 23, query_heads=1, state_heads=1, queries=1, states=1),
+    dict(dim=72, batch=1 << 22, query_heads=1, state_heads=1, queries=1, states=257),
+    dict(dim=128, batch=1 << 23, query_heads=1, state_heads=1, queries=0, states=1),
+    dict(dim=64, batch=1 << 24, query_heads=1, state_heads=1, queries=1, states=1),
+    dict(dim=256, batch=1 << 24, query_heads=1, state_heads=1, queries=1, states=1),
+    dict(dim=64, batch=1 << 20, query_heads=2, state_heads=1, queries=256, states=1),
+    dict(dim=128, batch=1 << 20, query_heads=2, state_heads=1, queries=128, states=1),
+    dict(dim=256, batch=1 << 20, query_heads=2, state_heads=1, queries=64, states=1),
+    dict(dim=64, batch=1 << 20, query_heads=16, state_heads=16, queries=129, states=1),
+])
+def test_backward_grids_that_are_refused_before_any_launch(bk, change):
+    status, text = _backward(bk, _shape(bk, **change))
+    assert status == bk.ERR_UNSUPPORTED and "too many rows" in text, text
+
+
+# Workgroups of up to 64 rows: 256 threads per 32 of them; of more rows: 512 threads per 256 of them, 256
+# per 128 above 128 dimensions.
+@pytest.mark.parametrize("change", [
+    dict(dim=64, batch=1 << 24, query_heads=1, state_heads=1, queries=1),
+    dict(dim=128, batch=1 << 23, query_heads=1, state_heads=1, queries=33),
+    dict(dim=64, batch=1 << 23, query_heads=1, state_heads=1, queries=65),
+    dict(dim=128, batch=1 << 22, query_heads=1, state_heads=1, queries=257),
+    dict(dim=256, batch=1 << 23, query_heads=1, state_heads=1, queries=129),
+])
+def test_forward_grids_that_are_refused_before_any_launch(bk, change):
+    shape = _shape(bk, **change)
+    one = _rows(bk, batch_stride=1 << 17, head_stride=1 << 17, row_stride=256)
+    status, text = _attend(bk, shape, one, one, one, one)
+    assert status == bk.ERR_UNSUPPORTED and "too many rows" in text, text
+    status, text = _read(bk, _cache(bk, dim=shape.dim, state_heads=shape.state_heads), shape, one, one)
+    assert status == bk.ERR_UNSUPPORTED and "too many rows" in text, text

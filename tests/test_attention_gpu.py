@@ -252,3 +252,18 @@ def test_scores_of_minus_infinity(bk, dev, dtype, rows):
     keys[0, 0, 77, 0] = 0.0
     out, lse = bk.cross_attention(queries, keys, values, mask=mask.to(dev))
     assert torch.equal(out, values[:, :, 77:78].expand_as(out)) and lse.isfinite().all()
+
+
+def test_more_rows_than_a_join_could_hold(bk, dev):
+    """2^26 rows and some: more than one launch of the kernel that joins ranges could take, which a call with
+    enough rows does not launch.  Against a call with the last rows only."""
+    rows = (1 << 26) + 5
+    queries = torch.empty((1, 1, rows, 8), dtype=torch.bfloat16, device=dev)
+    queries[:] = ref.made(31, (1, 1, 1, 8), torch.bfloat16).to(dev)
+    last = ref.made(32, (1, 1, 517, 8), torch.bfloat16).to(dev)
+    queries[:, :, -517:] = last
+    keys, values = (ref.made(s, (1, 1, 5, 8), torch.bfloat16).to(dev) for s in (33, 34))
+    out, lse = bk.cross_attention(queries, keys, values)
+    want, want_lse = bk.cross_attention(last, keys, values)
+    assert torch.equal(out[:, :, -517:], want) and torch.equal(lse[:, :, -517:], want_lse)
+    assert torch.equal(out[:, :, 1 << 25], out[:, :, 0]) and torch.equal(lse[:, :, 1 << 25], lse[:, :, 0])
