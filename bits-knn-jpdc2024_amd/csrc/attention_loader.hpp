@@ -115,7 +115,7 @@ struct state_loader
     // A lane's scales, ready for use.  States that take part are a block's first ones, so the first of a
     // sixteen has the scales of all that do; where it takes no part they are 1.  A key's scale
     // multiplies the factor from scores to exponents (at least the least normal number: a masked score
-    // of -inf stays one).  Of a value's scale the power of two goes into the decoded values, exactly
+    // of -inf stays one; at most the largest: a score of zero stays one).  Of a value's scale the power of two goes into the decoded values, exactly
     // (bf16 has the exponents), and the mantissa into the exponents of the weights; the sum of weights
     // takes it out again.
     __device__ __forceinline__ scales ready(const place& p, bool in) const
@@ -124,7 +124,7 @@ struct state_loader
         if constexpr (CACHE)
         {
             const float key = in ? p.key_scale * a.exponent_scale : 1.0F;
-            s.key_factor = key < 1.17549435e-38F ? 1.17549435e-38F : key;
+            s.key_factor = key < 1.17549435e-38F ? 1.17549435e-38F : (key > 3.402823466e38F ? 3.402823466e38F : key);
             s.value_scale = in ? p.value_scale : 1.0F;
             const float mantissa =
                 __builtin_bit_cast(float, (__builtin_bit_cast(u32, s.value_scale) & 0x007FFFFFU) | 0x3F800000U);

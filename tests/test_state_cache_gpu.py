@@ -357,3 +357,12 @@ def test_sequences_without_states_whatever_the_queries_hold(bk, dev, dtype, dim,
     out, lse = bk.cached_attention(queries.to(dev), cache, table.to(dev), counts.to(dev))
     assert (out[1:] == 0).all() and (lse[1:] == -math.inf).all()
     _check(bk, dev, queries[:1], cache, table[:1])
+
+
+@pytest.mark.parametrize("rows", [3, 65])
+def test_key_scales_that_overflow_with_the_scale(bk, dev, rows):
+    """A key's scale times the call's is beyond fp32: scores of zero stay zero."""
+    shape = (1, 1, 1, rows, 3, 64, 16)
+    cache, table = _cache(bk, dev, shape, 10)
+    cache.key_scales.fill_(2.0 ** 127)
+    _check(bk, dev, torch.zeros_like(_queries(shape, torch.bfloat16)), cache, table, scale=64.0)
