@@ -92,9 +92,10 @@ inline bool apart(std::int64_t dim, std::int64_t (&stride)[3], const std::int64_
     return true;
 }
 
-// Strides are looked at where their extent is above 1; the view gets 0 elsewhere.
+// Strides are looked at where their extent is above 1; the view gets 0 elsewhere.  value_bytes: of a
+// vector's value.
 inline int check_rows(const char* name, const char* what, const bitsknn_rows& r, const bitsknn_attention_shape& s,
-                      int heads, int rows, bool written, rows_view& view)
+                      int heads, int rows, bool written, rows_view& view, int value_bytes = 2)
 {
     const std::int64_t extent[3] = {s.batch, heads, rows};
     std::int64_t stride[3] = {r.batch_stride, r.head_stride, r.row_stride};
@@ -114,7 +115,7 @@ inline int check_rows(const char* name, const char* what, const bitsknn_rows& r,
     for (int i = 0; i < 3; ++i)
     {
         stride[i] = extent[i] > 1 ? stride[i] : 0;
-        if (stride[i] < 0 || stride[i] % 8 != 0)
+        if (stride[i] < 0 || stride[i] % (16 / value_bytes) != 0)
         {
             return fail(BITSKNN_ERR_INVALID, "%s: %s: vectors must start on 16-byte boundaries (strides %lld, %lld, %lld)",
                         name, what, static_cast<long long>(r.batch_stride), static_cast<long long>(r.head_stride),

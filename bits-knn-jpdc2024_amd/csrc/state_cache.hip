@@ -215,13 +215,14 @@ extern "C" int bitsknn_cache_store(const bitsknn_state_cache* cache, int32_t typ
     {
         return status;
     }
-    // the 16-bit types' checks hold for 32 bits too; a query head per state head fills the shape
+    // a 16-bit type and a query head per state head fill the shape
     const bitsknn_attention_shape s = {type == BITSKNN_F32 ? BITSKNN_BF16 : type, cache->dim, batch, cache->state_heads,
                                        cache->state_heads, 0, states, 1.0F};
+    const int bytes = type == BITSKNN_F32 ? 4 : 2;
     store_args a = {};
     status = check_shape(name, s);
-    status = status != BITSKNN_OK ? status : check_rows(name, "keys", *keys, s, s.state_heads, states, false, a.states[0]);
-    status = status != BITSKNN_OK ? status : check_rows(name, "values", *values, s, s.state_heads, states, false, a.states[1]);
+    status = status != BITSKNN_OK ? status : check_rows(name, "keys", *keys, s, s.state_heads, states, false, a.states[0], bytes);
+    status = status != BITSKNN_OK ? status : check_rows(name, "values", *values, s, s.state_heads, states, false, a.states[1], bytes);
     status = status != BITSKNN_OK ? status : check_table(name, table, table_stride, batch, states, view);
     if (status != BITSKNN_OK || batch == 0 || states == 0 || cache->blocks == 0)
     {

@@ -490,7 +490,8 @@ typedef struct bitsknn_state_cache
  * by it is exact and each value is rounded once, to the nearest e4m3 number (ties to even).  A NaN or an
  * infinity becomes the NaN code.  block_counts of the written blocks is set.
  *   type           BITSKNN_BF16, BITSKNN_FP16 or BITSKNN_F32: what keys and values hold
- *   keys, values   batch x cache->state_heads x states x cache->dim
+ *   keys, values   batch x cache->state_heads x states x cache->dim; vectors start on 16-byte boundaries
+ *                  (strides of whole eights, for BITSKNN_F32 of whole fours)
  *   counts         NULL, or batch int32 as for bitsknn_cross_attention
  *   table          batch rows of at least ceil(states / block) entries
  * Blocks behind a sequence's count, and the places of a block behind its last state, are left as they

@@ -228,3 +228,17 @@ def test_forward_grids_that_are_refused_before_any_launch(bk, change):
     assert status == bk.ERR_UNSUPPORTED and "too many rows" in text, text
     status, text = _read(bk, _cache(bk, dim=shape.dim, state_heads=shape.state_heads), shape, one, one)
     assert status == bk.ERR_UNSUPPORTED and "too many rows" in text, text
+
+
+def test_store_boundaries_by_type(bk):
+    """16-byte boundaries are strides of whole eights for the 16-bit types, of whole fours for float32."""
+    odd = _rows(bk, row_stride=68)
+    for kind in (bk.BF16, bk.FP16):
+        status, text = _store(bk, type=kind, keys=odd)
+        assert status == bk.ERR_INVALID and "keys: vectors must start on 16-byte boundaries" in text
+    for change in (dict(row_stride=66), dict(head_stride=1022), dict(batch_stride=(1 << 20) + 2)):
+        status, text = _store(bk, type=bk.F32, values=_rows(bk, **change))
+        assert status == bk.ERR_INVALID and "values: vectors must start on 16-byte boundaries" in text
+    # behind these boundaries, the next check speaks
+    status, text = _store(bk, type=bk.F32, keys=odd, values=odd, table=None)
+    assert status == bk.ERR_INVALID and "table: null pointer" in text

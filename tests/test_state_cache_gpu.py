@@ -366,3 +366,15 @@ def test_key_scales_that_overflow_with_the_scale(bk, dev, rows):
     cache, table = _cache(bk, dev, shape, 10)
     cache.key_scales.fill_(2.0 ** 127)
     _check(bk, dev, torch.zeros_like(_queries(shape, torch.bfloat16)), cache, table, scale=64.0)
+
+
+def test_float32_vectors_on_16_byte_boundaries(bk, dev):
+    """Strides of whole fours: 16 bytes, though not whole eights as the 16-bit types want them."""
+    wide = ref.made(20, (2, 3, 50, 24), torch.float32).to(dev)
+    odd = ref.made(21, (2, 3, 50, 12), torch.float32).to(dev)
+    table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+    for k, v in ((wide[..., :8], wide[..., 12:20]), (odd[..., :8], odd[..., 4:])):
+        one = bk.cache_store(bk.state_cache(8, 3, 16, 8, dev), k, v, table)
+        two = bk.cache_store(bk.state_cache(8, 3, 16, 8, dev), k.contiguous(), v.contiguous(), table)
+        for a, b in zip(one, two):
+            assert torch.equal(a, b)
