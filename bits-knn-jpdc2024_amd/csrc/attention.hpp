@@ -239,6 +239,9 @@ __device__ __forceinline__ vuint4 read_column(u32 first, u32 second)
     return vuint4{lo.x, lo.y, hi.x, hi.y};
 }
 
+// Between LDS writes and reads that lanes of one wave exchange: no instruction, an order for the compiler.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // ---- rows and states --------------------------------------------------------------------------
 
 // a value that all lanes hold, in a scalar register

@@ -1,4 +1,4 @@
-// Attention of few rows: the states are streamed once past at most 32 rows per state head.
+// Attention of few rows: the states are streamed past tiles of at most 32 rows.
 #ifndef BITSKNN_CSRC_ATTENTION_STREAM_HPP_
 #define BITSKNN_CSRC_ATTENTION_STREAM_HPP_
 
@@ -18,7 +18,8 @@ constexpr u32 STREAM_ROWS = 32;
 // pipeline over its tiles: while tile t is multiplied, the vectors of t + 1 are on their way into
 // registers, and so is what has to be known before the vectors of t + 2 can be asked for (mask; block,
 // its count and scales; the table entry of t + 3).  The vectors pass through LDS (the wave's own part)
-// to reach the operands' layout.
+// to reach the operands' layout.  A wave's LDS instructions are served in order, so lanes that exchange
+// values there need no barrier, only a fence that keeps the compiler from moving them.
 template <typename T, int DP, bool CACHE>
 __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attention_stream_kernel(const attention_args a)
 {
@@ -78,8 +79,10 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
     {
         const u32 taking = in;
         const typename wave_type::scales scales = w.ready(now, ((taking >> (lane % 32)) & 1) != 0);
+        wave_fence(); // behind the reads of the tile before
         w.template put<true>(keys, next_keys, 1.0F);
         w.template put<false>(values, next_values, scales.value_scale);
+        wave_fence();
         now = next;
         next.block = after.block;
         in = w.taking_part(now, tile + STREAM_WAVES);
@@ -173,6 +176,7 @@ __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attentio
     }
 
     // the waves' sums, row by row in LDS: 32 rows of DP floats fill a wave's part
+    wave_fence();
     weight += other_half(weight);
     if (half == 0)
     {

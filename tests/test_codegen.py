@@ -40,3 +40,52 @@ def test_streaming_loop_of_the_bits_kernel_is_wave_uniform(tmp_path):
                             timeout=600).stderr
     assert report.count("UniformityInfo for function") == 3
     assert "CYCLES WITH DIVERGENT EXIT" not in report
+
+
+STREAM = """
+#include "attention_stream.hpp"
+namespace bitsknn {
+void launch(const attention_args& a) {
+    attention_stream_kernel<__bf16, 64, false><<<1, 256>>>(a);
+    attention_stream_kernel<__bf16, 128, true><<<1, 256>>>(a);
+    attention_stream_kernel<_Float16, 256, false><<<1, 256>>>(a);
+}
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="needs hipcc")
+def test_lds_that_lanes_exchange_without_a_barrier_is_fenced(tmp_path):
+    """The stream kernel's waves pass tiles from lane to lane through LDS of their own, without a barrier.
+    Nothing but a fence tells the compiler that a lane reads what another has written, so in the kernel's IR
+    one lies between the stores to LDS and the reads from it, both ways."""
+    src = tmp_path / "inst.hip"
+    src.write_text(STREAM)
+    ir = tmp_path / "inst.ll"
+    subprocess.run(["hipcc", "-O3", "-std=c++20", "--offload-arch=gfx950", "-I", os.path.join(ROOT, "include"),
+                    "-I", CSRC, "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                    "-Wno-unused-command-line-argument", "-S", "-emit-llvm", "--cuda-device-only",
+                    "-o", str(ir), str(src)], check=True, capture_output=True, timeout=600)
+    kernels = 0
+    for body in ir.read_text().split("\ndefine ")[1:]:
+        body = body.split("\n}\n")[0]
+        if "attention_stream_kernel" not in body.split("\n")[0]:
+            continue
+        kernels += 1
+        last, stores, reads = None, 0, 0
+        for line in body.split("\n"):
+            if " fence " in " " + line.strip() or "amdgcn.s.barrier" in line:
+                last = None
+                continue
+            kind = None
+            if line.strip().startswith("store ") and "addrspace(3)" in line:
+                kind = "store"
+                stores += 1
+            elif "addrspace(3)" in line and (" = load " in line or "ds.read.tr" in line):
+                kind = "read"
+                reads += 1
+            if kind is not None:
+                assert last in (None, kind), (body.split("\n")[0], line)
+                last = kind
+        assert stores > 0 and reads > 0
+    assert kernels == 3
