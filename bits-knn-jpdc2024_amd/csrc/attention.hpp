@@ -73,7 +73,6 @@ struct attention_grad_args
     rows_view grad_keys;
     rows_view grad_values;
     float* delta;       // batch x query heads x rows: sum of grad_out * out
-    float* part;        // partial gradients of the keys and values of the row splits
     u32 key_tiles;
 };
 
@@ -259,18 +258,6 @@ __device__ __forceinline__ u32 state_count(const attention_args& a, u32 b)
     }
     const std::int32_t c = a.counts[b];
     return c <= 0 ? 0 : (static_cast<u32>(c) < a.states ? static_cast<u32>(c) : a.states);
-}
-
-// bit l: state first + l of sequence b takes part (all 64 lanes call it)
-__device__ __forceinline__ u64 states_taking_part(const attention_args& a, u32 b, u32 count, u32 first)
-{
-    const u32 j = first + (threadIdx.x & 63);
-    bool in = j < count;
-    if (a.mask != nullptr && in)
-    {
-        in = a.mask[static_cast<std::int64_t>(b) * a.mask_stride + j] != 0;
-    }
-    return __ballot(in);
 }
 
 // Row r of the rows that read state head `head` of sequence b: the query heads of the group one after
