@@ -3,7 +3,7 @@
 
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--only LEG,...] [--skip LEG,...]
                     [--k 32] [--block-size 256] [--items-per-thread 8] [--prefetch]
-                    [--fused-d D] [--fused-k K] [--fused-workspace-only] [--no-verify]
+                    [--fused-d D] [--fused-k K] [--fused-workspace-only] [--no-verify] [--details FILE]
 
 A step is one bits top-k pass (through the C ABI) over a resident 1024 x 1,048,576 fp32 matrix
 of i.i.d. uniform [0,1) values (4 GiB, generated on the device).  The printed JSON line follows
@@ -12,7 +12,8 @@ the reference's throughput convention: elements/s = rows*cols / mean step time
 bandwidth with its algorithmic bytes (4 B read per matrix element + 8 B written per output pair)
 over the kernel's mean duration measured with events on the launch stream.
 
-The same line carries the other workloads of the path, each leg with the fraction of the roofline
+The same line carries a `summary` of the other workloads of the path; --details writes the whole record
+(27 KB, more than a log's tail keeps of one line) to a file, each leg with the fraction of the roofline
 that bounds it (`frac`) and `verified`: after a leg's timed launches a sample of its rows or
 queries is compared with the CPU oracle (top-k: values and labels bit for bit; distances: k-th
 neighbour distance within 1e-5 of the scale of its terms and recall >= 0.999), so that a launch
@@ -608,6 +609,15 @@ def summarise(result):
     return out
 
 
+LINE = ("metric", "value", "unit", "n_gpus", "steps", "warmup", "ms_per_step", "higher_is_better", "scaling",
+        "vs_baseline", "dtype", "data", "config", "roofline", "verified", "cpu_baseline", "summary")
+
+
+def line_of(result):
+    """What the printed line holds of the record: the headline with its roofline and the summary of the rest."""
+    return {key: result[key] for key in LINE if key in result}
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -626,6 +636,7 @@ def main():
     ap.add_argument("--fused-workspace-only", action="store_true",
                     help="time the fused grid through the workspace entry point only (counter passes)")
     ap.add_argument("--no-verify", action="store_true", help="leave out the comparison with the oracle")
+    ap.add_argument("--details", default="", help="write the record of every leg to this file")
     args = ap.parse_args()
     if args.gpus != 1:
         print("bench.py: this build runs on exactly one GPU (--gpus 1); multi-GPU figures are not "
@@ -719,7 +730,10 @@ def main():
     if "cpu" in legs:
         result["cpu_baseline"] = leg_cpu(1024, 65536, 32)
     result["summary"] = summarise(result)
-    print(json.dumps(result))
+    if args.details:
+        with open(args.details, "w") as f:
+            json.dump(result, f)
+    print(json.dumps(line_of(result)))
 
 
 if __name__ == "__main__":
