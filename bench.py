@@ -655,7 +655,7 @@ def main():
     check = not args.no_verify
     oracle = None
     if check:
-        from oracle import binding as oracle  # the checker of every leg, never the thing measured
+        from oracle import binding as oracle  # what every leg is compared with, never the thing measured
         oracle.lib()
     dev = torch.device("cuda:0")
     torch.cuda.set_device(dev)

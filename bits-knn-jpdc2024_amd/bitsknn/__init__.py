@@ -464,6 +464,7 @@ def cross_attention(queries, keys, values, counts=None, mask=None, scale=None, o
     counts: None or batch int32, the states of each sequence; mask: None or batch x states bool / uint8,
     the states that take part; scale: None -> dim ** -0.5.  workspace: None -> allocated here; or a uint8
     device tensor (cross_attention_workspace_bytes; a smaller one is used as far as it goes).
+    torch's autograd does not see the call: gradients are those that cross_attention_backward returns.
     Returns (out, lse): out like queries, lse batch x query heads x rows float32."""
     batch, state_heads, states, dim = keys.shape
     device = queries.device
@@ -564,7 +565,8 @@ def _table_args(table, batch, device):
 def cache_store(cache, keys, values, table, counts=None):
     """Writes keys and values (batch x state heads x states x dim; bfloat16, float16 or float32) into the
     blocks of the cache that table (batch x at least ceil(states / block) int32) names
-    (bitsknn_cache_store).  counts: None or batch int32.  Returns the cache."""
+    (bitsknn_cache_store).  A block is written from its first state, with a new scale: to append to one,
+    store it again from all its states.  counts: None or batch int32.  Returns the cache."""
     import torch
     batch, state_heads, states, dim = keys.shape
     device = keys.device

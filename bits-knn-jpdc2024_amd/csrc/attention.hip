@@ -110,7 +110,8 @@ __device__ __forceinline__ u32 tile_order(const attention_args& a)
 // the values, and looks for the next scores' maximum.  The next tile's vectors are on their way into
 // registers while a tile is worked on; they are put into LDS (two tiles of keys, three of values, since
 // the slowest wave may still read the last values of the tile before) ahead of a tile's last step, which
-// already reads the next keys: one barrier per tile.
+// already reads the next keys: one barrier per tile.  Weights are rounded to 16 bits for the second product, as
+// the matrix instructions want them; their sum is taken before that.
 template <typename T, int DP, bool CACHE>
 __global__ void __launch_bounds__(64 * tile_waves(DP), DP <= 64 ? 4 : (DP <= 128 ? 2 : 1)) attention_tile_kernel(const attention_args a)
 {

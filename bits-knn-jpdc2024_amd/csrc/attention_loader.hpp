@@ -200,6 +200,9 @@ struct state_loader
         }
     }
 
+    // Decoded codes are two chunks per load: a row's even chunks are written by one instruction, the odd ones
+    // by the next, and two neighbouring rows meet in the same banks then (40 % of the LDS cycles of the cache's
+    // stream kernel, 15 % of its tile kernel's; neither is bound by LDS).  The caller's states meet none.
     template <bool KEY>
     __device__ __forceinline__ void put(char* tile, const vuint4 (&x)[LOADS], float scale) const
     {

@@ -19,7 +19,9 @@ constexpr u32 STREAM_ROWS = 32;
 // registers, and so is what has to be known before the vectors of t + 2 can be asked for (mask; block,
 // its count and scales; the table entry of t + 3).  The vectors pass through LDS (the wave's own part)
 // to reach the operands' layout.  A wave's LDS instructions are served in order, so lanes that exchange
-// values there need no barrier, only a fence that keeps the compiler from moving them.
+// values there need no barrier, only a fence that keeps the compiler from moving them.  (Heads of 136 to 256
+// dimensions: the query's operands and two tiles on their way do not fit beside the sums, 141 registers are
+// kept in scratch memory; 188 us, 5.7 TB/s, for 64 x 16/4 heads, one token over 4096 states x 256.)
 template <typename T, int DP, bool CACHE>
 __global__ void __launch_bounds__(64 * STREAM_WAVES, DP <= 128 ? 2 : 1) attention_stream_kernel(const attention_args a)
 {

@@ -385,7 +385,8 @@ int bitsknn_fused_status(void* stream);
  * the caller's (bitsknn_rows, in elements; an input's stride may be 0).  query_heads is a multiple of
  * state_heads: query head h reads state head h / (query_heads / state_heads).
  *   type           BITSKNN_BF16 or BITSKNN_FP16
- *   dim            1 <= dim <= 256, a multiple of 8; vectors start on 16-byte boundaries
+ *   dim            1 <= dim <= 256, a multiple of 8; vectors start on 16-byte boundaries, rows less than
+ *                  2^24 values apart
  *   queries        rows per query head, may be 0
  *   states         states per state head, may be 0
  *   scale          positive, and finite when multiplied by log2(e)
@@ -404,6 +405,9 @@ int bitsknn_fused_status(void* stream);
  * to the vectors' type for the second product, the result once at the end.
  * The launch depends on the sizes only, never on counts or mask, so a captured call may be replayed
  * with other contents.  Calls that overlap in time need workspaces of their own.
+ * BITSKNN_ERR_UNSUPPORTED for another type or dim, rows further apart, and sizes that a launch cannot hold
+ * (2^32 threads; 2^31 rows per state head); BITSKNN_ERR_INVALID for arguments that contradict the above.
+ * Everything is checked before the first launch.
  */
 #define BITSKNN_BF16 0
 #define BITSKNN_FP16 1
@@ -495,8 +499,9 @@ typedef struct bitsknn_state_cache
  *   counts         NULL, or batch int32 as for bitsknn_cross_attention
  *   table          batch rows of at least ceil(states / block) entries
  * Blocks behind a sequence's count, and the places of a block behind its last state, are left as they
- * were.  A table must not name a block twice (which of the writers a block then holds the states of,
- * is not defined).
+ * were.  A block is written from its first state, with a scale of its own each time: one that is to hold
+ * more states than it does is stored again from all of them.  A table must not name a block twice (which of
+ * the writers a block then holds the states of, is not defined).
  */
 #define BITSKNN_F32 2
 int bitsknn_cache_store(const bitsknn_state_cache* cache, int32_t type, int32_t batch, int32_t states,

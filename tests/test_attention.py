@@ -242,3 +242,29 @@ def test_store_boundaries_by_type(bk):
     # behind these boundaries, the next check speaks
     status, text = _store(bk, type=bk.F32, keys=odd, values=odd, table=None)
     assert status == bk.ERR_INVALID and "table: null pointer" in text
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_ranges_of_states(bk, dim):
+    """Ranges of at least 512 states up to 64 rows per state head, of at least 256 with more rows, no more
+    than give the GPU 512 or 256 workgroups, and no more than 64."""
+    size = bk.lib().bitsknn_cross_attention_workspace_bytes
+    padded = 64 * -(-dim // 64) if dim <= 128 else 256
+
+    def ranges(**kw):
+        shape = _shape(bk, dim=dim, **kw)
+        per = shape.batch * shape.query_heads * shape.queries * (4 * padded + 8)
+        assert size(shape) % per == 0
+        return size(shape) // per
+
+    few = dict(batch=1, query_heads=4, state_heads=2, queries=32)
+    assert ranges(states=1023, **few) == 0 and ranges(states=1024, **few) == 2
+    assert ranges(states=1 << 20, **few) == 64
+    many = dict(batch=1, query_heads=4, state_heads=2, queries=33)
+    assert ranges(states=511, **many) == 0 and ranges(states=512, **many) == 2
+    assert ranges(states=1 << 20, **many) == 64
+    # 256 and 128 workgroups already: one more each makes 512 and 256
+    assert ranges(states=1 << 20, batch=64, query_heads=8, state_heads=4, queries=1) == 2
+    assert ranges(states=1 << 20, batch=128, query_heads=8, state_heads=4, queries=1) == 0
+    assert ranges(states=1 << 20, batch=32, query_heads=8, state_heads=4, queries=33) == 2
+    assert ranges(states=1 << 20, batch=64, query_heads=8, state_heads=4, queries=33) == 0

@@ -267,3 +267,23 @@ def test_more_rows_than_a_join_could_hold(bk, dev):
     want, want_lse = bk.cross_attention(last, keys, values)
     assert torch.equal(out[:, :, -517:], want) and torch.equal(lse[:, :, -517:], want_lse)
     assert torch.equal(out[:, :, 1 << 25], out[:, :, 0]) and torch.equal(lse[:, :, 1 << 25], lse[:, :, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 70])
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 1e-20])
+def test_scales_near_zero(bk, dev, dtype, rows, scale):
+    """Below fp32's least normal number too: all states that take part count the same, the others nothing."""
+    queries, keys, values = _inputs(dev, (2, 2, 1, rows, 200, 64), dtype, 18)
+    mask = torch.rand((2, 200), generator=torch.Generator().manual_seed(6)) < 0.5
+    _check(bk, queries, keys, values, mask=mask.to(dev), scale=scale)
+
+
+def test_autograd_does_not_see_the_call(bk, dev):
+    """As documented: inputs that require gradients are taken, the result has no history."""
+    queries, keys, values = (x.requires_grad_() for x in _inputs(dev, (1, 2, 2, 3, 40, 64), torch.bfloat16))
+    out, lse = bk.cross_attention(queries, keys, values)
+    assert not out.requires_grad and not lse.requires_grad
+    grads = bk.cross_attention_backward(torch.ones_like(out), queries, keys, values, out, lse)
+    assert not any(x.requires_grad for x in grads)
+    assert "autograd does not see" in bk.cross_attention.__doc__
