@@ -730,10 +730,10 @@ def main():
     if "cpu" in legs:
         result["cpu_baseline"] = leg_cpu(1024, 65536, 32)
     result["summary"] = summarise(result)
+    print(json.dumps(line_of(result)), flush=True)
     if args.details:
         with open(args.details, "w") as f:
             json.dump(result, f)
-    print(json.dumps(line_of(result)))
 
 
 if __name__ == "__main__":

@@ -402,7 +402,9 @@ int bitsknn_fused_status(void* stream);
  *                  bitsknn_cross_attention_workspace_bytes returns what the call wants.  NULL or a
  *                  smaller workspace is not an error: fewer ranges, down to one.
  * Products are summed in fp32 and softmax statistics are fp32; the weights exp(s - maximum) are rounded
- * to the vectors' type for the second product, the result once at the end.
+ * to the vectors' type for the second product, the result once at the end.  Weights reach 2^8 before the
+ * sums are divided by theirs, so bf16 values beyond 2^119 / states may overflow the sums, and scores beyond
+ * 2^127 are infinite.
  * The launch depends on the sizes only, never on counts or mask, so a captured call may be replayed
  * with other contents.  Calls that overlap in time need workspaces of their own.
  * BITSKNN_ERR_UNSUPPORTED for another type or dim, rows further apart, and sizes that a launch cannot hold
@@ -448,8 +450,8 @@ int bitsknn_cross_attention(const bitsknn_attention_shape* shape, const bitsknn_
  * queries' gradient the derivatives enter in two pieces), sums are fp32 and the results are rounded once.
  * Fp16: derivatives of the scores below 2^-24 vanish, so gradients want a loss scale that keeps them
  * above it.  There is no such limit above: derivatives beyond 65504 are held times a power of two, and a
- * gradient is infinite only where it is itself beyond fp16 (workgroups that meet such derivatives walk their
- * part twice).  No gradient may share memory with an input.
+ * gradient is infinite only where it is itself beyond fp16 (workgroups that meet such derivatives, or
+ * gradients that are not finite, walk their part twice).  No gradient may share memory with an input.
  */
 size_t bitsknn_cross_attention_backward_workspace_bytes(const bitsknn_attention_shape* shape);
 int bitsknn_cross_attention_backward(const bitsknn_attention_shape* shape, const bitsknn_rows* grad_out,
